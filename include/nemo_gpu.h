@@ -147,6 +147,108 @@ int nemo_lstm_cell(const float *gates, const float *c_in, float *c_out, float *h
 int nemo_joint_argmax(const float *enc, int64_t enc_ld, const float *pred, int64_t pred_ld, const uint16_t *W,
                       const float *bias, int V, int H, int rows, int *out_idx, float *out_val, void *stream);
 
+/* ---- operators of streaming state-space layers -------------------------------------------------
+   The reference has none of these: they serve checkpoints whose projections are held in 4 bits and
+   whose sequence mixer carries a fixed state (causal convolution + selective scan) instead of a K/V
+   window. Activations may be fp32, bf16 or fp16 (NEMO_ELT_*); sums and states are fp32 and a value
+   is rounded once, to nearest even, where it is stored. Values, small tensors and states need the
+   alignment of their type; rows whose base and pitch are 16-byte aligned are moved 16 bytes at a
+   time. Buffers that are written must not overlap others unless stated. Nothing is allocated and
+   nothing synchronises; calls may be captured into graphs and may run on several streams at once. */
+enum { NEMO_ELT_F32 = 0, NEMO_ELT_BF16 = 1, NEMO_ELT_F16 = 2 };
+
+/* MXFP4 rows. A block is 32 consecutive columns of a row; its scale is 2^e with e = floor(log2 of
+   its largest magnitude) - 2, not below 2^-127, held as the byte e + 127; a value is its e2m1 code
+   (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) times the scale, rounded to nearest, ties to the
+   even code, beyond 6 to 6. A block that holds an infinity or a NaN gets the byte 255 (NaN) and zero
+   codes. Codes: two a byte, the even column in the low nibble, rows ldq bytes apart. Scales: tiles
+   of 128 rows x 4 blocks, byte (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 of tile
+   (r / 128) * ceil(K / 128) + b / 4 for row r and block b; nemo_mxfp4_scale_bytes(rows, K) bytes.
+   The quantiser writes the bytes of its rows (those of a last, partly filled tile of columns as 0)
+   and leaves the bytes of rows past the last one alone. K: a multiple of 32. */
+int64_t nemo_mxfp4_scale_bytes(int64_t rows, int64_t K);
+int nemo_mxfp4_quantize(const void *X, int x_elt, int64_t ldx, int64_t rows, int64_t K, uint8_t *codes, int64_t ldq, uint8_t *scales, void *stream);
+/* The values that codes and scales stand for (rounded to y_elt; a NaN scale gives NaN). */
+int nemo_mxfp4_dequantize(const uint8_t *codes, int64_t ldq, const uint8_t *scales, int64_t rows, int64_t K, void *Y, int y_elt, int64_t ldy, void *stream);
+
+/* C[m][n] (= or +=) alpha * act(sum_k A[m][k] W[n][k] + bias[n]) for MXFP4 rows A [M][K] and W [N][K]
+   on the block-scaled tensor cores: products are exact, sums fp32. The epilogue is nemo_gemm's: bias
+   -> act -> alpha -> store or accumulate (fp32 C only); NEMO_ACT_GLU pairs columns n and n + N/2 into
+   N/2 outputs, a * sigmoid(b), and needs N to be a multiple of 256. K: a positive multiple of 32. Codes,
+   scales and code pitches 16-byte aligned. Scale bytes of the columns past K must not be 255 (the
+   quantiser writes 0); those of the rows past M or N may hold anything. */
+typedef struct {
+    const uint8_t *A;
+    int64_t lda;              /* bytes */
+    const uint8_t *a_scales;
+    const uint8_t *W;
+    int64_t ldw;              /* bytes */
+    const uint8_t *w_scales;
+    const float *bias;        /* [N] or NULL */
+    void *C;
+    int64_t ldc;              /* elements */
+    int c_elt;
+    int M, N, K;
+    int act, accumulate;
+    float alpha;
+} nemo_gemm_mxfp4_args_t;
+int nemo_gemm_mxfp4(const nemo_gemm_mxfp4_args_t *a, void *stream);
+
+/* Causal depthwise convolution over the rows of `streams` independent streams, with carried history:
+   y[t][d] = act(bias[d] + sum_j w[d][j] * u[t + j]), u = the taps - 1 history rows, then the x rows.
+   Stream s has lens[s] rows (device ints, taken into 0..c; NULL: c each); rows of y behind its last
+   one are left as they were. hist_in [streams][taps-1][D] (NULL: zeros) holds the rows before this
+   call's, hist_out the last taps - 1 rows of u after it (NULL: not kept); they may be the same
+   buffer. taps 1..8; act NEMO_ACT_NONE or NEMO_ACT_SILU. One row per stream is the single-token form. */
+typedef struct {
+    const void *x;
+    int64_t x_ld, x_sstride;
+    const float *w;           /* [D][taps] */
+    const float *bias;        /* [D] or NULL */
+    const void *hist_in;
+    void *hist_out;
+    void *y;
+    int64_t y_ld, y_sstride;
+    const int *lens;
+    int streams, c, D, taps;
+    int elt;                  /* of x, y and the history */
+    int act;
+} nemo_causal_conv_args_t;
+int nemo_causal_conv(const nemo_causal_conv_args_t *a, void *stream);
+
+/* Selective state-space scan over the rows of `streams` independent streams, with carried state.
+   With step = dt[t][d] + dt_bias[d] (softplus of it where dt_softplus) and group g = d / (D / groups):
+     h[d][n] = exp(step * A[d][n]) * h[d][n] + step * x[t][d] * B[t][g][n]
+     y[t][d] = (sum_n h[d][n] * C[t][g][n] + skip[d] * x[t][d]) * silu(z[t][d])
+   z, skip and dt_bias may be NULL (no gate, 0, 0). Rows of B and C hold groups * N elements. Stream s
+   has lens[s] rows (device ints, taken into 0..c; NULL: c each); rows of y behind its last one are
+   left as they were. state_in [streams][D][N] (NULL: zeros), state_out the state after the last row
+   (of no rows: the state before; NULL: not kept); they may be the same buffer. N 1..128, D a
+   multiple of groups. One row per stream is the single-token form. */
+typedef struct {
+    const void *x;
+    int64_t x_ld, x_sstride;
+    const void *dt;
+    int64_t dt_ld, dt_sstride;
+    const void *z;
+    int64_t z_ld, z_sstride;
+    const void *B;
+    const void *C;
+    int64_t bc_ld, bc_sstride;
+    const float *A;           /* [D][N] */
+    const float *skip;
+    const float *dt_bias;
+    int dt_softplus;
+    const float *state_in;
+    float *state_out;
+    void *y;
+    int64_t y_ld, y_sstride;
+    const int *lens;
+    int streams, c, D, N, groups;
+    int elt;                  /* of x, dt, z, B, C and y */
+} nemo_selective_scan_args_t;
+int nemo_selective_scan(const nemo_selective_scan_args_t *a, void *stream);
+
 const char *nemo_gpu_last_error(void);
 /* 0 if no kernel has reported a device-side failure (a bounded wait that gave up instead of
    hanging); otherwise -1 with the message in nemo_gpu_last_error(). Synchronous (reads a flag);

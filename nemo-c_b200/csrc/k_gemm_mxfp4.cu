@@ -1,0 +1,435 @@
+// GEMM of MXFP4 rows: C[m][n] (=, +=) alpha * act(sum_k A[m][k] W[n][k] + bias[n]), both operands
+// as 4-bit codes with a power-of-two scale per 32 columns. tcgen05.mma (kind::mxf4, block-scaled)
+// multiplies the codes as they are: every product of two codes and two scales is exact, the sums
+// are fp32 in tensor memory, and nothing is rounded before the epilogue.
+//
+// Orientation: weight rows are the MMA's 128-row side (tensor-memory lanes), activation rows its
+// columns, so that one kernel serves one row and thousands: a warp's 32 lanes hold 32 neighbouring
+// output columns of an output row, and each store of the epilogue is one contiguous run.
+//
+// A unit of work is WT weight tiles of 128 rows (two for GLU: value rows n and gate rows n + N/2;
+// two also for many activation rows, which then cross L2 -> SM once for 256 weight rows) by one
+// tile of BN activation rows. One stage holds 256 columns of k: the weight and activation codes,
+// brought in by TMA with the 128-byte swizzle, and their scale tiles, one bulk copy each. The MMA
+// thread copies the scales from shared to tensor memory (tcgen05.cp; each stage has tensor-memory
+// columns of its own, so a later stage's copy never meets an MMA that still reads them) and issues
+// four MMAs of 64 columns per weight tile.
+//
+// Few units: a cluster of 2, 4 or 8 CTAs splits k; the partial tiles meet in shared memory across
+// the cluster and are added in the order of their ranks, so results do not depend on scheduling.
+// Otherwise persistent CTAs walk the units, the epilogue of one running beside the MMAs of the
+// next. Warp roles (320 threads): warp 0 loads, warp 1 owns tensor memory and issues the MMAs,
+// warps 2-9 run the epilogue. Every wait on a barrier is bounded: on a timeout the CTA records an
+// error, takes part in the remaining cluster barriers and unwinds.
+#include <cuda.h>
+#include <cstring>
+#include <atomic>
+#include "elt.cuh"
+#include "mxfp4.cuh"
+#include "sm100.cuh"
+
+extern "C" int *nb_tc_error_ptr(void);
+
+namespace {
+
+constexpr int BM = 128;   // weight rows per tile
+constexpr int BKB = 128;  // code bytes per row and stage: 256 columns of k, one swizzle span
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int ATOM = 512; // bytes of one scale tile (128 rows x 128 columns of k)
+
+struct MxArgs {
+    const uint8_t *as, *ws;  // scales
+    const float *bias;
+    void *C;
+    int64_t ldc;
+    int M, N, K, kblocks, katoms, splits, kb_per_split, n_wtiles, n_mtiles, units, act, accumulate;
+    float alpha;
+    int *err;
+};
+
+template <int BN, int WT>
+struct Cfg {
+    static constexpr int W_BYTES = BM * BKB, A_BYTES = BN * BKB;
+    static constexpr int WS_OFF = WT * W_BYTES + A_BYTES;      // scales: 2 atoms per weight tile, 2 for the activations
+    static constexpr int STAGE = WS_OFF + (WT + 1) * 2 * ATOM;
+    static constexpr int STAGES = BN == 128 ? (WT == 2 ? 4 : 6) : (WT == 2 ? 4 : 8);
+    static constexpr int SLOTS = WT == 1 ? 2 : BN == 128 ? 3 : 4;  // accumulators of BN columns
+    static constexpr int SC_COLS = (WT + 1) * 8;                 // scale columns per stage
+    static constexpr int COLS = SLOTS * BN + STAGES * SC_COLS;
+    static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
+    static_assert(COLS <= 512, "tensor memory");
+    static_assert(STAGE % 1024 == 0, "swizzled tiles start on 1 KB");
+    static_assert(WT * BN * BM * 4 <= STAGES * STAGE, "partial tiles reuse the stages");
+};
+
+__device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(bytes),
+                 "r"(sm100::smem_u32(bar))
+                 : "memory");
+}
+
+// Descriptor of a scale tile in shared memory: 32 rows of 16 bytes, contiguous, no swizzle (core
+// matrices of 8 rows x 16 bytes are 128 bytes apart).
+__device__ __forceinline__ uint64_t desc_scale(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+// 32 lanes x 16 bytes, written to all four 32-lane quarters of tensor memory.
+__device__ __forceinline__ void cp_scale(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Instruction descriptor, kind::mxf4: e2m1 x e2m1 with ue8m0 scales, both operands K-major. An
+// MMA takes two scales per row out of a word of four: half 0 or half 1 of it.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int N, int half) {
+    return ((uint32_t)(half * 2) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(BM >> 7) << 27) |
+           ((uint32_t)(half * 2) << 29);
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// bias -> act -> alpha -> store or accumulate, one output element.
+template <typename T>
+__device__ __forceinline__ void finish(const MxArgs &p, int m, int n, float va, float vb, float ba, float bb) {
+    float v = va + ba;
+    if (p.act == NEMO_ACT_GLU)
+        v *= nb::sigmoid_fast(vb + bb);
+    else if (p.act == NEMO_ACT_SILU)
+        v *= nb::sigmoid_fast(v);
+    else if (p.act == NEMO_ACT_RELU)
+        v = v < 0.0f ? 0.0f : v;  // a NaN stays one
+    v *= p.alpha;
+    T *c = (T *)p.C + (int64_t)m * p.ldc + n;
+    if (p.accumulate) v += nb::to_f32(*c);
+    *c = nb::from_f32<T>(v);
+}
+
+template <typename T, int BN, int WT>
+__global__ void __launch_bounds__(THREADS, 1)
+    gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const __grid_constant__ MxArgs p) {
+    using C = Cfg<BN, WT>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *stages = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = (uint64_t *)(stages + C::STAGES * C::STAGE);
+    uint64_t *empty = full + C::STAGES;
+    uint64_t *acc_full = empty + C::STAGES;     // [SLOTS] MMA -> epilogue
+    uint64_t *acc_empty = acc_full + C::SLOTS;  // [SLOTS] epilogue -> MMA
+    uint32_t *tmem_holder = (uint32_t *)(acc_empty + C::SLOTS);
+    volatile int *flags = (volatile int *)(tmem_holder + 1);  // [0] a wait gave up, [1] the epilogue's own
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) { sm100::mbar_init(&full[s], 1); sm100::mbar_init(&empty[s], 1); }
+        for (int s = 0; s < C::SLOTS; ++s) { sm100::mbar_init(&acc_full[s], 1); sm100::mbar_init(&acc_empty[s], 1); }
+        flags[0] = flags[1] = 0;
+        sm100::fence_mbar_init();
+        sm100::tma_prefetch_desc(&tmW);
+        sm100::tma_prefetch_desc(&tmA);
+    }
+    if (warp == 1) {
+        sm100::tmem_alloc(tmem_holder, C::TMEM_COLS);
+        sm100::tmem_relinquish();
+    }
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    nb::pdl_wait();
+
+    const bool glu = p.act == NEMO_ACT_GLU;
+    const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
+    const int u0 = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x, ustep = p.splits > 1 ? p.units : gridDim.x;
+    const int kb0 = rank * p.kb_per_split, kb1 = min(p.kblocks, kb0 + p.kb_per_split);
+    // first weight row of tile i of unit u
+    auto wrow = [&](int wt, int i) { return glu ? wt * BM + (i ? p.N / 2 : 0) : (wt * WT + i) * BM; };
+
+    if (warp == 0 && lane == 0) {
+        int it = 0;
+        for (int u = u0; u < p.units && !flags[0]; u += ustep) {
+            const int mt = u % p.n_mtiles, wt = u / p.n_mtiles;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % C::STAGES;
+                if (it >= C::STAGES && !sm100::mbar_wait(&empty[s], ((it / C::STAGES) - 1) & 1)) { flags[0] = 1; atomicExch(p.err, 5); break; }
+                if (flags[0]) break;
+                uint8_t *st = stages + s * C::STAGE;
+                const uint32_t sb = (uint32_t)min(2, p.katoms - kb * 2) * ATOM;  // scale tiles of these columns
+                // a second weight tile wholly past the last row is not loaded (its output is not written)
+                const bool two = WT == 2 && wrow(wt, 1) < p.N;
+                sm100::mbar_arrive_expect_tx(&full[s], (two ? 2 : 1) * (C::W_BYTES + sb) + C::A_BYTES + sb);
+#pragma unroll
+                for (int i = 0; i < WT; ++i) {
+                    if (i && !two) break;
+                    const int r = wrow(wt, i);
+                    sm100::tma_load_2d(st + i * C::W_BYTES, &tmW, &full[s], kb * BKB, r);
+                    bulk_g2s(st + C::WS_OFF + i * 2 * ATOM, p.ws + ((int64_t)(r / BM) * p.katoms + kb * 2) * ATOM, sb, &full[s]);
+                }
+                sm100::tma_load_2d(st + WT * C::W_BYTES, &tmA, &full[s], kb * BKB, mt * BN);
+                bulk_g2s(st + C::WS_OFF + WT * 2 * ATOM, p.as + ((int64_t)(mt * BN / 128) * p.katoms + kb * 2) * ATOM, sb, &full[s]);
+            }
+        }
+        // a launch that gave up waits for its own copies before its shared memory goes away
+        if (flags[0])
+            for (int j = max(0, it - C::STAGES); j < it; ++j) sm100::mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, 100000000LL);
+    } else if (warp == 1 && lane == 0) {
+        int it = 0, t = 0;
+        for (int u = u0; u < p.units && !flags[0]; u += ustep, ++t) {
+            const int wt = u / p.n_mtiles;
+            const bool two = WT == 2 && wrow(wt, 1) < p.N;
+            bool ok = true;
+#pragma unroll
+            for (int i = 0; i < WT; ++i) {
+                const int q = t * WT + i;
+                if (q >= C::SLOTS && !sm100::mbar_wait(&acc_empty[q % C::SLOTS], ((q / C::SLOTS) - 1) & 1)) ok = false;
+            }
+            if (!ok) { flags[0] = 1; atomicExch(p.err, 6); break; }
+            sm100::tc_fence_after();
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % C::STAGES;
+                if (!sm100::mbar_wait(&full[s], (it / C::STAGES) & 1)) { flags[0] = 1; atomicExch(p.err, 7); break; }
+                sm100::tc_fence_after();
+                const uint32_t st = sm100::smem_u32(stages + s * C::STAGE);
+                const uint32_t sc = tmem + C::SLOTS * BN + s * C::SC_COLS;
+                const int atoms = min(2, p.katoms - kb * 2), steps = min(4, (p.K - kb * 256 + 63) / 64);
+#pragma unroll
+                for (int i = 0; i <= WT; ++i) {  // weight tiles, then the activations
+                    if (i == 1 && WT == 2 && !two) continue;
+                    for (int a = 0; a < atoms; ++a) cp_scale(sc + i * 8 + a * 4, desc_scale(st + C::WS_OFF + (i * 2 + a) * ATOM));
+                }
+#pragma unroll
+                for (int i = 0; i < WT; ++i) {
+                    if (i && !two) break;
+                    const uint32_t d = tmem + ((t * WT + i) % C::SLOTS) * BN;
+                    for (int kk = 0; kk < steps; ++kk)
+                        mma_mxf4(d, sm100::desc_k_sw128(st + i * C::W_BYTES + kk * 32), sm100::desc_k_sw128(st + WT * C::W_BYTES + kk * 32),
+                                 idesc_mxf4(BN, kk & 1), sc + i * 8 + (kk >> 1) * 4, sc + WT * 8 + (kk >> 1) * 4, kb != kb0 || kk != 0);
+                }
+                sm100::mma_commit(&empty[s]);
+            }
+#pragma unroll
+            for (int i = 0; i < WT; ++i) sm100::mma_commit(&acc_full[(t * WT + i) % C::SLOTS]);
+        }
+    } else if (warp >= 2) {
+        const int q = warp & 3, half = (warp - 2) >> 2;  // the 32 lanes and the half of the columns of this warp
+        const int row = q * 32 + lane, etid = threadIdx.x - 64;
+        constexpr int HALF = BN >= 32 ? BN / 2 : BN;
+        const int jbeg = half * HALF, jend = half * HALF < BN ? jbeg + HALF : jbeg;
+        const int nout = glu ? p.N / 2 : p.N;
+        int t = 0;
+        for (int u = u0; u < p.units; u += ustep, ++t) {
+            const int mt = u % p.n_mtiles, wt = u / p.n_mtiles, m0 = mt * BN, mcount = min(BN, p.M - m0);
+            bool good = true;
+#pragma unroll
+            for (int i = 0; i < WT; ++i)
+                if (!sm100::mbar_wait(&acc_full[(t * WT + i) % C::SLOTS], ((t * WT + i) / C::SLOTS) & 1)) good = false;
+            if (!good) { flags[1] = 1; flags[0] = 1; atomicExch(p.err, 8); }
+            // flags[1] is written only by epilogue threads before this barrier: all of them decide alike
+            sm100::named_barrier(1, 256);
+            if (flags[1]) break;
+            sm100::tc_fence_after();
+            const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+            if (p.splits > 1) {  // partial tiles to shared memory: [tile][column][lane]
+                float *part = (float *)stages;
+#pragma unroll
+                for (int i = 0; i < WT; ++i)
+                    for (int j0 = jbeg; j0 < jend && j0 < mcount; j0 += 16) {
+                        float v[16];
+                        sm100::tmem_ld16(lanes + ((t * WT + i) % C::SLOTS) * BN + j0, v);
+#pragma unroll
+                        for (int jj = 0; jj < 16; ++jj) part[(i * BN + j0 + jj) * BM + row] = v[jj];
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < WT; ++i) {
+                    if (i && glu) break;
+                    const int n = (glu ? wt * BM : wrow(wt, i)) + row;
+                    const bool on = n < nout;
+                    const float ba = on && p.bias ? p.bias[n] : 0.0f, bb = on && glu && p.bias ? p.bias[n + p.N / 2] : 0.0f;
+                    const uint32_t acc = lanes + ((t * WT + i) % C::SLOTS) * BN, gate = lanes + ((t * WT + 1) % C::SLOTS) * BN;
+                    for (int j0 = jbeg; j0 < jend && j0 < mcount; j0 += 16) {
+                        float v[16], g[16];
+                        sm100::tmem_ld16(acc + j0, v);
+                        if (WT == 2 && glu) sm100::tmem_ld16(gate + j0, g);
+                        if (on)
+#pragma unroll
+                            for (int jj = 0; jj < 16; ++jj)
+                                if (j0 + jj < mcount) finish<T>(p, m0 + j0 + jj, n, v[jj], WT == 2 ? g[jj] : 0.0f, ba, bb);
+                    }
+                }
+                sm100::tc_fence_before();
+                sm100::named_barrier(1, 256);
+                if (etid < WT) mbar_arrive(&acc_empty[(t * WT + etid) % C::SLOTS]);
+            }
+        }
+    }
+    __syncwarp();
+    if (p.splits > 1) {
+        // one unit per cluster: each rank adds and finishes its share of the columns
+        __syncthreads();
+        cluster_sync();
+        const int mt = u0 % p.n_mtiles, wt = u0 / p.n_mtiles, m0 = mt * BN, mcount = min(BN, p.M - m0);
+        const int nout = glu ? p.N / 2 : p.N, total = (glu || WT == 1 ? 1 : WT) * mcount * BM;
+        const uint32_t part = sm100::smem_u32(stages);
+        if (!flags[0])
+            for (int e = rank * THREADS + threadIdx.x; e < total; e += p.splits * THREADS) {
+                const int row = e % BM, j = e / BM % mcount, i = e / BM / mcount;
+                const int n = (glu ? wt * BM : wrow(wt, i)) + row;
+                if (n >= nout) continue;
+                float v = 0.0f, g = 0.0f;
+                for (int r = 0; r < p.splits; ++r) {
+                    v += ld_cluster(part + ((i * BN + j) * BM + row) * 4, r);
+                    if (WT == 2 && glu) g += ld_cluster(part + ((BN + j) * BM + row) * 4, r);
+                }
+                finish<T>(p, m0 + j, n, v, g, p.bias ? p.bias[n] : 0.0f, glu && p.bias ? p.bias[n + p.N / 2] : 0.0f);
+            }
+        cluster_sync();  // no CTA leaves while another reads its shared memory
+    }
+    sm100::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        sm100::tc_fence_after();
+        sm100::tmem_dealloc(tmem, C::TMEM_COLS);
+    }
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+    static std::atomic<EncodeTiled> fn{nullptr};
+    EncodeTiled f = fn.load();
+    if (!f) {
+        void *q = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) != cudaSuccess || !q) return nullptr;
+        fn.store(f = (EncodeTiled)q);
+    }
+    return f;
+}
+
+// Codes as bytes: [rows][K / 2], boxes of 128 bytes by box_rows; columns past K / 2 read as zero.
+int code_map(CUtensorMap *m, const uint8_t *base, int64_t K, int64_t rows, int64_t ld, int box_rows) {
+    EncodeTiled f = encoder();
+    if (!f) return nb_set_error("nemo_gemm_mxfp4: cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[2] = { (cuuint64_t)(K / 2), (cuuint64_t)rows };
+    cuuint64_t strides[1] = { (cuuint64_t)ld };
+    cuuint32_t box[2] = { (cuuint32_t)BKB, (cuuint32_t)box_rows };
+    cuuint32_t es[2] = { 1, 1 };
+    CUresult r = f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return nb_set_error("nemo_gemm_mxfp4: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return 0;
+}
+
+template <typename T, int BN, int WT>
+int run(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
+    using C = Cfg<BN, WT>;
+    const bool glu = a->act == NEMO_ACT_GLU;
+    CUtensorMap mw, ma;
+    if (code_map(&mw, a->W, a->K, a->N, a->ldw, BM) || code_map(&ma, a->A, a->K, a->M, a->lda, BN)) return -1;
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return nb_set_error("nemo_gemm_mxfp4: no CUDA device");
+    MxArgs p;
+    memset(&p, 0, sizeof p);
+    p.as = a->a_scales; p.ws = a->w_scales; p.bias = a->bias; p.C = a->C; p.ldc = a->ldc;
+    p.M = a->M; p.N = a->N; p.K = a->K; p.act = a->act; p.accumulate = a->accumulate; p.alpha = a->alpha;
+    p.kblocks = (a->K + 255) / 256;
+    p.katoms = (a->K + 127) / 128;
+    const int wspan = glu ? BM : WT * BM;
+    p.n_wtiles = ((glu ? a->N / 2 : a->N) + wspan - 1) / wspan;
+    p.n_mtiles = (a->M + BN - 1) / BN;
+    const int64_t units = (int64_t)p.n_wtiles * p.n_mtiles;
+    if (units > 0x3fffffff) return nb_set_error("nemo_gemm_mxfp4: too many tiles");
+    p.units = (int)units;
+    // k is split while the CTAs of all units still fit the SMs at once and each keeps a stage
+    int splits = 1;
+    while (splits < 8 && p.units * splits * 2 <= sms && splits * 2 <= p.kblocks) splits *= 2;
+    p.kb_per_split = (p.kblocks + splits - 1) / splits;
+    while (splits > 1 && (splits - 1) * p.kb_per_split >= p.kblocks) {  // every rank has k-blocks
+        splits /= 2;
+        p.kb_per_split = (p.kblocks + splits - 1) / splits;
+    }
+    p.splits = splits;
+    p.err = nb_tc_error_ptr();
+    if (!p.err) return nb_set_error("nemo_gemm_mxfp4: device error word unavailable");
+    auto kernel = gemm_mxfp4_kernel<T, BN, WT>;
+    if (nb_smem_attr((const void *)kernel, C::SMEM)) return -1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits > 1 ? p.units * splits : p.units < sms ? p.units : sms);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (nb_pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (splits > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = splits;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    cudaLaunchKernelEx(&cfg, kernel, mw, ma, p);
+    return nb_check_launch("gemm_mxfp4_kernel");
+}
+
+template <typename T>
+int by_rows(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
+    const bool glu = a->act == NEMO_ACT_GLU;
+    if (a->M <= 16) return glu ? run<T, 16, 2>(a, st) : run<T, 16, 1>(a, st);
+    if (a->M <= 64) return glu ? run<T, 64, 2>(a, st) : run<T, 64, 1>(a, st);
+    return glu ? run<T, 128, 2>(a, st) : run<T, 128, 1>(a, st);
+}
+
+}  // namespace
+
+extern "C" int nemo_gemm_mxfp4(const nemo_gemm_mxfp4_args_t *a, void *stream) {
+    if (!a) return nb_set_error("nemo_gemm_mxfp4: null arguments");
+    if (a->M < 0 || a->N < 0 || a->K < 0) return nb_set_error("nemo_gemm_mxfp4: bad shape M=%d N=%d K=%d", a->M, a->N, a->K);
+    if (a->act < NEMO_ACT_NONE || a->act > NEMO_ACT_GLU) return nb_set_error("nemo_gemm_mxfp4: unknown activation %d", a->act);
+    if (!nb::elt_ok(a->c_elt)) return nb_set_error("nemo_gemm_mxfp4: unknown element type %d", a->c_elt);
+    if (a->K == 0 || a->K % 32) return nb_set_error("nemo_gemm_mxfp4: K=%d must be a positive multiple of 32", a->K);
+    if (a->act == NEMO_ACT_GLU && a->N % 256) return nb_set_error("nemo_gemm_mxfp4: GLU needs N=%d to be a multiple of 256 (whole scale tiles in each half)", a->N);
+    if (a->accumulate && a->c_elt != NEMO_ELT_F32) return nb_set_error("nemo_gemm_mxfp4: accumulate needs an fp32 output");
+    if (a->M == 0 || a->N == 0) return 0;
+    if (!a->A || !a->a_scales || !a->W || !a->w_scales || !a->C) return nb_set_error("nemo_gemm_mxfp4: null pointer");
+    if (((uintptr_t)a->A | (uintptr_t)a->W | (uintptr_t)a->a_scales | (uintptr_t)a->w_scales) & 15 || a->lda % 16 || a->ldw % 16)
+        return nb_set_error("nemo_gemm_mxfp4: codes, scales and code row pitches must be 16-byte aligned");
+    if (a->lda < a->K / 2 || a->ldw < a->K / 2) return nb_set_error("nemo_gemm_mxfp4: code row pitches below K / 2 bytes");
+    if (a->M > 1 && a->ldc < (a->act == NEMO_ACT_GLU ? a->N / 2 : a->N)) return nb_set_error("nemo_gemm_mxfp4: ldc below the output columns");
+    if ((uintptr_t)a->C % nb::elt_size(a->c_elt) || (uintptr_t)a->bias % 4) return nb_set_error("nemo_gemm_mxfp4: C and bias must be aligned to their type");
+    int rc = 0;
+    NB_ELT_SWITCH(a->c_elt, T, rc = by_rows<T>(a, (cudaStream_t)stream));
+    return rc;
+}

@@ -1199,6 +1199,17 @@ extern "C" int nemo_gpu_wait_selftest(int kind, long long limit_cycles, void *st
 // been left dirty, and the allocation-free entry clears its own again before its next launch.
 static std::atomic<unsigned> g_tc_error_reports{0};
 
+// Address of the error word on the current device, for the tensor-core kernels of other files.
+extern "C" int *nb_tc_error_ptr(void) {
+    static std::atomic<int *> at[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+    int *p = dev < 64 ? at[dev].load() : nullptr;
+    if (!p && cudaGetSymbolAddress((void **)&p, g_tc_error) != cudaSuccess) return nullptr;
+    if (dev < 64) at[dev].store(p);
+    return p;
+}
+
 extern "C" int nemo_gpu_check_device_errors(void) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_tc_error, sizeof v) != cudaSuccess) return nb_set_error("cannot read the device error flag");

@@ -38,6 +38,26 @@ class GemmArgs(C.Structure):  # nemo_gemm_args_t
                 ("alpha", C.c_float), ("c32", C.c_void_p), ("ldc32", C.c_int64)]
 
 
+class GemmMxfp4Args(C.Structure):  # nemo_gemm_mxfp4_args_t
+    _fields_ = [("A", C.c_void_p), ("lda", C.c_int64), ("a_scales", C.c_void_p), ("W", C.c_void_p), ("ldw", C.c_int64), ("w_scales", C.c_void_p),
+                ("bias", C.c_void_p), ("C", C.c_void_p), ("ldc", C.c_int64), ("c_elt", C.c_int), ("M", C.c_int), ("N", C.c_int), ("K", C.c_int),
+                ("act", C.c_int), ("accumulate", C.c_int), ("alpha", C.c_float)]
+
+
+class CausalConvArgs(C.Structure):  # nemo_causal_conv_args_t
+    _fields_ = [("x", C.c_void_p), ("x_ld", C.c_int64), ("x_sstride", C.c_int64), ("w", C.c_void_p), ("bias", C.c_void_p), ("hist_in", C.c_void_p),
+                ("hist_out", C.c_void_p), ("y", C.c_void_p), ("y_ld", C.c_int64), ("y_sstride", C.c_int64), ("lens", C.c_void_p), ("streams", C.c_int),
+                ("c", C.c_int), ("D", C.c_int), ("taps", C.c_int), ("elt", C.c_int), ("act", C.c_int)]
+
+
+class SelectiveScanArgs(C.Structure):  # nemo_selective_scan_args_t
+    _fields_ = [("x", C.c_void_p), ("x_ld", C.c_int64), ("x_sstride", C.c_int64), ("dt", C.c_void_p), ("dt_ld", C.c_int64), ("dt_sstride", C.c_int64),
+                ("z", C.c_void_p), ("z_ld", C.c_int64), ("z_sstride", C.c_int64), ("B", C.c_void_p), ("C", C.c_void_p), ("bc_ld", C.c_int64),
+                ("bc_sstride", C.c_int64), ("A", C.c_void_p), ("skip", C.c_void_p), ("dt_bias", C.c_void_p), ("dt_softplus", C.c_int),
+                ("state_in", C.c_void_p), ("state_out", C.c_void_p), ("y", C.c_void_p), ("y_ld", C.c_int64), ("y_sstride", C.c_int64),
+                ("lens", C.c_void_p), ("streams", C.c_int), ("c", C.c_int), ("D", C.c_int), ("N", C.c_int), ("groups", C.c_int), ("elt", C.c_int)]
+
+
 def lib():
     global _lib
     if _lib is None:
@@ -130,6 +150,13 @@ def _setup_api(L):
     L.nemo_flatten_rows.argtypes = [vp, vp, vp] + [C.c_int] * 5 + [vp]
     L.nemo_lstm_cell.argtypes = [vp, vp, vp, vp, C.c_int, C.c_int, vp]
     L.nemo_joint_argmax.argtypes = [vp, i64, vp, i64, vp, vp, C.c_int, C.c_int, C.c_int, vp, vp, vp]
+    L.nemo_mxfp4_scale_bytes.argtypes = [i64, i64]
+    L.nemo_mxfp4_scale_bytes.restype = i64
+    L.nemo_mxfp4_quantize.argtypes = [vp, C.c_int, i64, i64, i64, vp, i64, vp, vp]
+    L.nemo_mxfp4_dequantize.argtypes = [vp, i64, vp, i64, i64, vp, C.c_int, i64, vp]
+    L.nemo_gemm_mxfp4.argtypes = [C.POINTER(GemmMxfp4Args), vp]
+    L.nemo_causal_conv.argtypes = [C.POINTER(CausalConvArgs), vp]
+    L.nemo_selective_scan.argtypes = [C.POINTER(SelectiveScanArgs), vp]
     L.nemo_gpu_last_error.restype = C.c_char_p
     L.nemo_gpu_launch_count.restype = C.c_uint64
     L.nemoasr_mel_create.restype = C.c_void_p

@@ -24,6 +24,7 @@
 #include <cuda.h>
 #include <cstring>
 #include <atomic>
+#include "cluster.cuh"
 #include "elt.cuh"
 #include "mxfp4.cuh"
 #include "sm100.cuh"
@@ -98,23 +99,6 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uin
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
-    uint32_t a;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-}
-
 // bias -> act -> alpha -> store or accumulate, one output element.
 template <typename T>
 __device__ __forceinline__ void finish(const MxArgs &p, int m, int n, float va, float vb, float ba, float bb) {
@@ -164,7 +148,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     nb::pdl_wait();
 
     const bool glu = p.act == NEMO_ACT_GLU;
-    const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
+    const int rank = p.splits > 1 ? (int)nb::cluster_rank() : 0;
     const int u0 = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x, ustep = p.splits > 1 ? p.units : gridDim.x;
     const int kb0 = rank * p.kb_per_split, kb1 = min(p.kblocks, kb0 + p.kb_per_split);
     // first weight row of tile i of unit u
@@ -292,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (p.splits > 1) {
         // one unit per cluster: each rank adds and finishes its share of the columns
         __syncthreads();
-        cluster_sync();
+        nb::cluster_sync();
         const int mt = u0 % p.n_mtiles, wt = u0 / p.n_mtiles, m0 = mt * BN, mcount = min(BN, p.M - m0);
         const int nout = glu ? p.N / 2 : p.N, total = (glu || WT == 1 ? 1 : WT) * mcount * BM;
         const uint32_t part = sm100::smem_u32(stages);
@@ -303,12 +287,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (n >= nout) continue;
                 float v = 0.0f, g = 0.0f;
                 for (int r = 0; r < p.splits; ++r) {
-                    v += ld_cluster(part + ((i * BN + j) * BM + row) * 4, r);
-                    if (WT == 2 && glu) g += ld_cluster(part + ((BN + j) * BM + row) * 4, r);
+                    v += nb::ld_cluster(part + ((i * BN + j) * BM + row) * 4, r);
+                    if (WT == 2 && glu) g += nb::ld_cluster(part + ((BN + j) * BM + row) * 4, r);
                 }
                 finish<T>(p, m0 + j, n, v, g, p.bias ? p.bias[n] : 0.0f, glu && p.bias ? p.bias[n + p.N / 2] : 0.0f);
             }
-        cluster_sync();  // no CTA leaves while another reads its shared memory
+        nb::cluster_sync();  // no CTA leaves while another reads its shared memory
     }
     sm100::tc_fence_before();
     __syncthreads();

@@ -2,14 +2,27 @@
 //
 //   h[d][n] = exp(step A[d][n]) h[d][n] + step x[d] B[n],   y[d] = (sum_n h[d][n] C[n] + skip[d] x[d]) silu(z[d])
 //
-// The state is held in fp32 registers: LPC lanes share a channel, four states each, so that a
-// warp reads the state of its channels as one contiguous run and a row's sum over the states is a few
-// shuffles.
+// The state is held in fp32 registers: LPC lanes share a channel, NS states each, so that a warp
+// reads the state of its channels as one contiguous run. What belongs to a (row, channel) and not to
+// a state (the step with its softplus, the gate, the output) is computed once, by one lane for the
+// others, and the sums over the states of V rows are folded together: V values over LPC lanes take
+// about V shuffles, and each row's sum ends in the lane that writes it.
+//
+// Two kernels. Few rows: the state's bytes (8 N per channel) dominate, the kernel is bound by HBM;
+// warps load everything of their rows at once and nothing is staged. Many rows: bound by the
+// exponentials (one per row, channel and state on the special-function units, 16 a clock an SM); half
+// of a block's warps prepare tiles of rows in shared memory and write the finished ones out while
+// the other half runs the recurrence.
+#include <type_traits>
+#include <cstdlib>
 #include "elt.cuh"
+#include "cluster.cuh"
+
+static int nb_scan_want() { const char *e = getenv("WANT"); return e ? atoi(e) : 148 * 32; }
+static int nb_scan_split() { const char *e = getenv("SPLIT"); return e ? atoi(e) : 148 * 5; }
 
 namespace {
 
-constexpr int NT = 128;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct ScanArgs {
@@ -20,119 +33,545 @@ struct ScanArgs {
     void *y;
     int64_t y_ld, y_ss;
     const int *lens;
-    int streams, c, D, N, per_group, softplus, wps;  // channels per group, warps per stream
-    int64_t warps;
+    int streams, c, D, N, per_group, softplus;
+    int tiles, units;  // a warp's worth of channels: of a group, of a stream
+    int64_t items;     // few rows: warps; many rows: channel tiles of all streams
+    int tw, ranks;     // many rows: chunks of time in a block, blocks of a cluster
 };
 
-// log(1 + e^v); for v > 20 that is v to fp32
-__device__ __forceinline__ float softplus_f(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
+__device__ __forceinline__ float ex2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// log(1 + e^v) = max(v, 0) + log1p(e), e = exp(-|v|) <= 1, and log1p(e) = 2 artanh(e / (2 + e)): the
+// argument is at most 1/3, so seven terms of the series leave 1.4e-8 of it. No cancellation at either end.
+__device__ __forceinline__ float softplus_f(float v) {
+    const float e = ex2(-fabsf(v) * LOG2E);
+    const float s = __fdividef(e, 2.0f + e), q = s * s;
+    float p = 1.0f / 13.0f;
+    p = fmaf(p, q, 1.0f / 11.0f);
+    p = fmaf(p, q, 1.0f / 9.0f);
+    p = fmaf(p, q, 1.0f / 7.0f);
+    p = fmaf(p, q, 1.0f / 5.0f);
+    p = fmaf(p, q, 1.0f / 3.0f);
+    p = fmaf(p * q, s, s);
+    return fmaf(2.0f, p, fmaxf(v, 0.0f));
+}
+
+// ---- few rows --------------------------------------------------------------------------------
+// A warp owns 32 / LPC channels. STEP (one row per stream): V streams at a time, their rows taken
+// together, so that V states are in flight per channel and A is read once for them. Otherwise: one
+// stream, V rows at a time.
+constexpr int FEW_NT = 128;
+
+template <typename T, int LPC, bool V4, bool STEP>
+__global__ void __launch_bounds__(FEW_NT) scan_few_kernel(const __grid_constant__ ScanArgs a) {
+    constexpr int CPW = 32 / LPC, V = LPC < 4 ? LPC : 4, REP = LPC / V;
+    nb::pdl_wait();
+    const int64_t w = ((int64_t)blockIdx.x * FEW_NT + threadIdx.x) >> 5;
+    if (w >= a.items) return;
+    const int lane = threadIdx.x & 31, sub = lane % LPC, n0 = sub * 4, v = sub / REP;  // this lane's states, and its row of V
+    const int64_t sblk = w / a.units;
+    const int unit = (int)(w - sblk * a.units), grp = unit / a.tiles;
+    const int dg = (unit - grp * a.tiles) * CPW + lane / LPC;
+    const bool on = dg < a.per_group;
+    const int d = grp * a.per_group + (on ? dg : a.per_group - 1);
+    const bool st4 = n0 < a.N;
+
+    auto load4 = [&](const float *p, float (&o)[4]) {
+        if (V4) {
+            if (st4) {
+                const float4 t = *(const float4 *)p;
+                o[0] = t.x; o[1] = t.y; o[2] = t.z; o[3] = t.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n0 + j < a.N) o[j] = p[j];
+        }
+    };
+    auto loadbc = [&](const T *p, float (&o)[4]) {
+        if (V4) {
+            if (st4) {
+                const nb::Vec<T, 4> t = *(const nb::Vec<T, 4> *)p;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = nb::to_f32(t.v[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n0 + j < a.N) o[j] = nb::to_f32(p[j]);
+        }
+    };
+    auto store4 = [&](float *p, const float (&o)[4]) {
+        if (V4) {
+            if (st4) *(float4 *)p = make_float4(o[0], o[1], o[2], o[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n0 + j < a.N) p[j] = o[j];
+        }
+    };
+
+    const int64_t s0 = STEP ? sblk * V : sblk;
+    constexpr int H = STEP ? V : 1;
+    float h[H][4], A2[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+    for (int r = 0; r < H; ++r) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[r][j] = 0.0f;
+        if (a.state_in && s0 + r < a.streams) load4(a.state_in + ((s0 + r) * a.D + d) * (int64_t)a.N + n0, h[r]);
+    }
+    load4(a.A + (int64_t)d * a.N + n0, A2);
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, skip = a.skip ? a.skip[d] : 0.0f;
+    const int64_t bc0 = (int64_t)grp * a.N + n0;
+    const int len = STEP ? 1 : a.lens ? max(0, min(a.lens[s0], a.c)) : a.c;
+
+    for (int t0 = 0; t0 < len; t0 += V) {
+        // this lane's row: of stream s0 + v (STEP), or row t0 + v
+        const int64_t s = STEP ? s0 + v : s0;
+        const int t = STEP ? 0 : t0 + v;
+        const bool live = STEP ? s < a.streams && (!a.lens || a.lens[s] > 0) : t < len;
+        float xv = 0.0f, step = 0.0f, gate = 1.0f;
+        if (live) {
+            xv = nb::to_f32(((const T *)a.x)[s * a.x_ss + t * a.x_ld + d]);
+            step = nb::to_f32(((const T *)a.dt)[s * a.dt_ss + t * a.dt_ld + d]);
+            if (a.z) gate = nb::to_f32(((const T *)a.z)[s * a.z_ss + t * a.z_ld + d]);
+        }
+        float b[V][4], c[V][4];
+#pragma unroll
+        for (int r = 0; r < V; ++r) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[r][j] = c[r][j] = 0.0f;
+            const int64_t at = STEP ? (s0 + r) * a.bc_ss + bc0 : s0 * a.bc_ss + (t0 + r) * a.bc_ld + bc0;
+            if (STEP ? s0 + r < a.streams : t0 + r < len) {
+                loadbc((const T *)a.B + at, b[r]);
+                loadbc((const T *)a.C + at, c[r]);
+            }
+        }
+        if (live) {
+            step += bias;
+            if (a.softplus) step = softplus_f(step);
+            if (a.z) gate *= nb::sigmoid_fast(gate);
+        }
+        const float sx = step * xv;
+        float sum[V];
+#pragma unroll
+        for (int r = 0; r < V; ++r) {
+            const float sr = __shfl_sync(0xffffffffu, step, r * REP, LPC) * LOG2E, xr = __shfl_sync(0xffffffffu, sx, r * REP, LPC);
+            const bool go = STEP ? __shfl_sync(0xffffffffu, (int)live, r * REP, LPC) != 0 : t0 + r < len;
+            sum[r] = 0.0f;
+            if (go) {
+                float (&hh)[4] = h[STEP ? r : 0];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    hh[j] = fmaf(ex2(sr * A2[j]), hh[j], xr * b[r][j]);
+                    sum[r] = fmaf(hh[j], c[r][j], sum[r]);
+                }
+            }
+        }
+        nb::WarpFold<V, LPC / 2>::run(sum, lane);
+        if (live && on && sub % REP == 0) {
+            const float o = fmaf(skip, xv, sum[0]) * gate;
+            ((T *)a.y)[s * a.y_ss + t * a.y_ld + d] = nb::from_f32<T>(o);
+        }
+    }
+    if (a.state_out && on)
+#pragma unroll
+        for (int r = 0; r < H; ++r)
+            if (s0 + r < a.streams) store4(a.state_out + ((s0 + r) * a.D + d) * (int64_t)a.N + n0, h[r]);
+}
 
 template <typename T, int LPC, bool V4>
-__global__ void __launch_bounds__(NT) selective_scan_kernel(const __grid_constant__ ScanArgs a) {
-    constexpr int CPW = 32 / LPC;  // channels per warp
+int run_few(ScanArgs a, cudaStream_t st) {
+    constexpr int CPW = 32 / LPC, V = LPC < 4 ? LPC : 4;
+    a.tiles = (a.per_group + CPW - 1) / CPW;
+    a.units = a.D / a.per_group * a.tiles;
+    const bool step = a.c == 1;
+    a.items = (step ? (a.streams + V - 1) / V : a.streams) * (int64_t)a.units;
+    const int64_t blocks = (a.items * 32 + FEW_NT - 1) / FEW_NT;
+    if (blocks > 0x7fffffff) return nb_set_error("nemo_selective_scan: too many streams");
+    nb::launch(step ? scan_few_kernel<T, LPC, V4, true> : scan_few_kernel<T, LPC, V4, false>, dim3((unsigned)blocks), FEW_NT, 0, st, a);
+    return nb_check_launch("scan_few_kernel");
+}
+
+// ---- many rows -------------------------------------------------------------------------------
+
+typedef unsigned long long f2;  // two fp32 in a register pair
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 dup2(float v) { return pack2(v, v); }
+__device__ __forceinline__ float rcp(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// softplus_f of two values
+__device__ __forceinline__ f2 softplus2(f2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    const f2 e = pack2(ex2(-fabsf(a) * LOG2E), ex2(-fabsf(b) * LOG2E));
+    float u, w;
+    unpack2(add2(e, dup2(2.0f)), u, w);
+    const f2 s = mul2(e, pack2(rcp(u), rcp(w))), q = mul2(s, s);
+    f2 p = dup2(1.0f / 13.0f);
+    p = fma2(p, q, dup2(1.0f / 11.0f));
+    p = fma2(p, q, dup2(1.0f / 9.0f));
+    p = fma2(p, q, dup2(1.0f / 7.0f));
+    p = fma2(p, q, dup2(1.0f / 5.0f));
+    p = fma2(p, q, dup2(1.0f / 3.0f));
+    p = fma2(mul2(p, q), s, s);
+    return fma2(dup2(2.0f), p, pack2(fmaxf(a, 0.0f), fmaxf(b, 0.0f)));
+}
+
+// A lane owns a channel's whole state where N <= 16 (else LPC lanes, 16 states each, with the rows'
+// steps and outputs dealt out among them), so steps, gates and sums never leave its registers; only B
+// and C, shared by the warp's channels, pass through shared memory. A warp runs one chunk of rows of its
+// channels. Where the channels alone do not fill the GPU, time is cut as well: TW warps of a block
+// and R blocks of a cluster hold chunks of the same channels. Each chunk but the last finds the state
+// it ends in when started from zero, and the sum of its steps (all chunks start at once; the first
+// one starts from the true state and is done). A chunk's true first state is then folded from those
+// before it, h <- exp(A sum of steps) h + end, and the chunks run again from it, writing y. Nothing
+// but shared memory is needed for that, and the order of the sums is fixed.
+constexpr int LW = 8;  // warps per block
+template <int LPC>
+constexpr int tile_rows() { return LPC < 4 ? 4 : LPC; }  // at least one row per lane of a channel
+
+template <typename T, int LPC, int NS, bool V4>
+__global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_constant__ ScanArgs a) {
+    constexpr int U = tile_rows<LPC>(), CPW = 32 / LPC, NP = LPC * NS, RP = U / LPC;  // channels per warp, padded states, rows per lane and tile
+    constexpr int QUADS = U * NP / 4, QL = (QUADS + 31) / 32;   // groups of four states in a tile, per lane
+    extern __shared__ __align__(16) float smem[];  // [LW][2][U][NP]: the warps' tiles of B and C
+    float *ends = smem + LW * 2 * U * NP;          // [LW + 1][NS + 1][32]: end states and sums of steps of the warps' chunks, of the whole block
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPC, n0 = sub * NS;
     nb::pdl_wait();
-    const int64_t w = ((int64_t)blockIdx.x * NT + threadIdx.x) >> 5;
-    if (w >= a.warps) return;
-    const int lane = threadIdx.x & 31, n0 = (lane % LPC) * 4;
-    const int64_t s = w / a.wps;
-    const int d = (int)(w - s * a.wps) * CPW + lane / LPC;
-    const bool on = d < a.D;
-    const int dd = on ? d : a.D - 1;
-    const int len = a.lens ? max(0, min(a.lens[s], a.c)) : a.c;
-    float A2[4], h[4];
-    const int64_t sat = (s * a.D + dd) * (int64_t)a.N + n0;
+    const int rank = a.ranks > 1 ? blockIdx.x % a.ranks : 0;
+    const int64_t item = (blockIdx.x / a.ranks) * (int64_t)(LW / a.tw) + warp / a.tw;  // (stream, channel tile)
+    const bool real = item < a.items;
+    const int64_t s = real ? item / a.units : 0;
+    const int unit = real ? (int)(item - s * a.units) : 0, grp = unit / a.tiles;
+    const int dg = (unit - grp * a.tiles) * CPW + lane / LPC;
+    const bool on = real && dg < a.per_group;
+    const int64_t d = grp * a.per_group + min(dg, a.per_group - 1);
+    const int len = !real ? 0 : a.lens ? max(0, min(a.lens[s], a.c)) : a.c;
+    const int chunks = a.tw * a.ranks, chunk = rank * a.tw + warp % a.tw;
+    const int rows = (len + chunks * U - 1) / (chunks * U) * U;  // rows per chunk, whole tiles
+    const int tb = min(len, chunk * rows), te = min(len, tb + rows);
+
+    f2 A2[NS / 2], h[NS / 2];
+    const int64_t at = (s * a.D + d) * a.N + n0;
+    auto load_states = [&](const float *p, f2 (&o)[NS / 2]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) A2[j] = h[j] = 0.0f;
-    if (V4) {
-        if (n0 < a.N) {
-            const float4 t = *(const float4 *)(a.A + (int64_t)dd * a.N + n0);
-            A2[0] = t.x; A2[1] = t.y; A2[2] = t.z; A2[3] = t.w;
-            if (a.state_in) {
-                const float4 u = *(const float4 *)(a.state_in + sat);
-                h[0] = u.x; h[1] = u.y; h[2] = u.z; h[3] = u.w;
+        for (int j = 0; j < NS / 2; j += 2) {
+            float f[4];
+            if (V4 && n0 + 2 * j < a.N) {
+                const float4 v = *(const float4 *)(p + 2 * j);
+                f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) f[k] = !V4 && n0 + 2 * j + k < a.N ? p[2 * j + k] : 0.0f;
+            }
+            o[j] = pack2(f[0], f[1]);
+            o[j + 1] = pack2(f[2], f[3]);
+        }
+    };
+    load_states(a.A + d * a.N + n0, A2);
+#pragma unroll
+    for (int j = 0; j < NS / 2; ++j) h[j] = 0;
+    if (chunk == 0 && a.state_in) load_states(a.state_in + at, h);
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, skip = a.skip ? a.skip[d] : 0.0f;
+    const T *X = (const T *)a.x + s * a.x_ss + d, *DT = (const T *)a.dt + s * a.dt_ss + d;
+    const T *Z = a.z ? (const T *)a.z + s * a.z_ss + d : nullptr;
+    T *Y = (T *)a.y + s * a.y_ss + d;
+    const T *B = (const T *)a.B + s * a.bc_ss + (int64_t)grp * a.N, *C = (const T *)a.C + s * a.bc_ss + (int64_t)grp * a.N;
+    typedef float Tile[U][NP];
+    Tile &sb = ((Tile *)smem)[2 * warp], &sc = ((Tile *)smem)[2 * warp + 1];
+
+    // The chunk's rows: WRITE with the outputs, otherwise the end state and the sum of the steps alone.
+    auto pass = [&](auto write) __attribute__((always_inline)) {
+        constexpr bool WRITE = decltype(write)::value;
+        float total = 0.0f;
+        T rx[RP], rd[RP], rz[RP];
+        nb::Vec<T, 4> rb[QL], rc[QL];
+        // this lane's next rows of x, dt, z and its groups of B and C
+        const T *px = X + (int64_t)(tb + sub * RP) * a.x_ld, *pd = DT + (int64_t)(tb + sub * RP) * a.dt_ld;
+        const T *pz = WRITE && Z ? Z + (int64_t)(tb + sub * RP) * a.z_ld : nullptr;
+        T *py = Y + (int64_t)(tb + sub * RP) * a.y_ld;
+        const int64_t bc0 = (int64_t)(tb + lane / (NP / 4)) * a.bc_ld + lane % (NP / 4) * 4;
+        const T *pb = B + bc0, *pc = C + bc0;
+        auto fetch = [&](int left) __attribute__((always_inline)) {  // left: rows of the chunk from this tile on
+            const bool all = left >= U;
+#pragma unroll
+            for (int r = 0; r < RP; ++r) {
+                if (all || sub * RP + r < left) {
+                    rx[r] = px[r * a.x_ld];
+                    rd[r] = pd[r * a.dt_ld];
+                    if (WRITE && Z) rz[r] = pz[r * a.z_ld];
+                }
+            }
+            px += U * a.x_ld;
+            pd += U * a.dt_ld;
+            if (WRITE && Z) pz += U * a.z_ld;
+#pragma unroll
+            for (int k = 0; k < QL; ++k) {
+                // group e = lane + 32 k of the tile: row e / (NP / 4) of it, state e % (NP / 4) * 4
+                constexpr int QR = NP / 4;
+                const int e = lane + k * 32, row = e / QR, n = e % QR * 4;
+                const bool is = e < QUADS && (all || row < left);
+                const int64_t off = QR >= 32 ? (int64_t)(row - lane / QR) * a.bc_ld + (n - lane % QR * 4) : (int64_t)(k * 32 / QR) * a.bc_ld;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) rb[k].v[j] = rc[k].v[j] = nb::from_f32<T>(0.0f);
+                if (V4) {
+                    if (is && n < a.N) {
+                        rb[k] = *(const nb::Vec<T, 4> *)(pb + off);
+                        if (WRITE) rc[k] = *(const nb::Vec<T, 4> *)(pc + off);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (is && n + j < a.N) {
+                            rb[k].v[j] = pb[off + j];
+                            if (WRITE) rc[k].v[j] = pc[off + j];
+                        }
+                }
+            }
+            pb += U * a.bc_ld;
+            pc += U * a.bc_ld;
+        };
+        if (tb < te) fetch(te - tb);
+        for (int t0 = tb; t0 < te; t0 += U) {
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < QL; ++k) {
+                const int e = lane + k * 32;
+                if (e < QUADS) {
+                    const int r = e / (NP / 4), n = e % (NP / 4) * 4;
+                    *(float4 *)&sb[r][n] = make_float4(nb::to_f32(rb[k].v[0]), nb::to_f32(rb[k].v[1]), nb::to_f32(rb[k].v[2]), nb::to_f32(rb[k].v[3]));
+                    if (WRITE)
+                        *(float4 *)&sc[r][n] = make_float4(nb::to_f32(rc[k].v[0]), nb::to_f32(rc[k].v[1]), nb::to_f32(rc[k].v[2]), nb::to_f32(rc[k].v[3]));
+                }
+            }
+            float xv[RP], step[RP], sx[RP], gate[RP];
+#pragma unroll
+            for (int r = 0; r < RP; ++r) {
+                xv[r] = nb::to_f32(rx[r]);
+                step[r] = nb::to_f32(rd[r]) + bias;
+                if (WRITE && Z) gate[r] = nb::to_f32(rz[r]);
+            }
+            const int live = te - t0;  // rows of this tile that exist
+            if (live > U) fetch(live - U);
+            if (a.softplus) {
+#pragma unroll
+                for (int r = 0; r + 1 < RP; r += 2) unpack2(softplus2(pack2(step[r], step[r + 1])), step[r], step[r + 1]);
+                if (RP == 1) step[0] = softplus_f(step[0]);
+            }
+#pragma unroll
+            for (int r = 0; r < RP; ++r) {
+                const bool is = sub * RP + r < live;  // a row behind the last one keeps the state: a step and an input of 0
+                sx[r] = is ? step[r] * xv[r] : 0.0f;
+                step[r] = is ? step[r] * LOG2E : 0.0f;
+                if (WRITE && Z) gate[r] *= nb::sigmoid_fast(gate[r]);
+            }
+            __syncwarp();
+            float sum[U];
+#pragma unroll
+            for (int r = 0; r < U; ++r) {
+                const float st = LPC == 1 ? step[r % RP] : __shfl_sync(0xffffffffu, step[r % RP], r / RP, LPC);
+                const float in = LPC == 1 ? sx[r % RP] : __shfl_sync(0xffffffffu, sx[r % RP], r / RP, LPC);
+                const f2 st2 = dup2(st), in2 = dup2(in);
+                asm volatile("" ::: "memory");  // one row's B and C in registers at a time
+                if (!WRITE) total += st;
+                f2 acc = 0;
+#pragma unroll
+                for (int q = 0; q < NS / 4; ++q) {
+                    const float4 bv = *(const float4 *)&sb[r][n0 + 4 * q];
+                    float4 cv;
+                    if (WRITE) cv = *(const float4 *)&sc[r][n0 + 4 * q];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        f2 &hh = h[2 * q + j];
+                        float e0, e1;
+                        unpack2(mul2(st2, A2[2 * q + j]), e0, e1);
+                        hh = fma2(pack2(ex2(e0), ex2(e1)), hh, mul2(in2, j ? pack2(bv.z, bv.w) : pack2(bv.x, bv.y)));
+                        if (WRITE) {
+                            const f2 cc = j ? pack2(cv.z, cv.w) : pack2(cv.x, cv.y);
+                            acc = q + j ? fma2(hh, cc, acc) : mul2(hh, cc);
+                        }
+                    }
+                }
+                float lo, hi;
+                unpack2(acc, lo, hi);
+                sum[r] = lo + hi;
+            }
+            if (WRITE) {
+                nb::WarpFold<U, LPC / 2>::run(sum, lane);  // lane sub: rows sub * RP ..
+#pragma unroll
+                for (int r = 0; r < RP; ++r) {
+                    if (on && sub * RP + r < live) {
+                        float v = fmaf(skip, xv[r], sum[r]);
+                        if (Z) v *= gate[r];
+                        py[r * a.y_ld] = nb::from_f32<T>(v);
+                    }
+                }
+                py += U * a.y_ld;
             }
         }
+        return total;
+    };
+
+    if (chunks > 1) {
+        float *mine = ends + warp * (NS + 1) * 32 + lane, *block = ends + LW * (NS + 1) * 32 + lane;
+        auto put = [&](float *to, float total) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < NS / 2; ++j) {
+                float lo, hi;
+                unpack2(h[j], lo, hi);
+                to[2 * j * 32] = lo;
+                to[(2 * j + 1) * 32] = hi;
+            }
+            to[NS * 32] = total;
+        };
+        // h <- exp(A sum) h + end of a chunk (or of a block's chunks), given how to read it
+        auto fold = [&](auto get) __attribute__((always_inline)) {
+            const f2 t2 = dup2(get(NS));
+#pragma unroll
+            for (int j = 0; j < NS / 2; ++j) {
+                float e0, e1;
+                unpack2(mul2(t2, A2[j]), e0, e1);
+                h[j] = fma2(pack2(ex2(e0), ex2(e1)), h[j], pack2(get(2 * j), get(2 * j + 1)));
+            }
+        };
+        float total = 0.0f;
+        if (chunk < chunks - 1) total = pass(std::false_type{});
+        put(mine, total);
+        __syncthreads();
+        auto fold_warps = [&](int w0, int w1) __attribute__((always_inline)) {
+            for (int w = w0; w < w1; ++w) {
+                const float *e = ends + w * (NS + 1) * 32 + lane;
+                fold([&](int k) { return e[k * 32]; });
+                total += e[NS * 32];
+            }
+        };
+        if (a.ranks > 1) {  // one channel tile per block
+            if (warp == LW - 1 && rank < a.ranks - 1) {
+                total = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NS / 2; ++j) h[j] = 0;
+                fold_warps(0, LW);
+                put(block, total);
+            }
+            nb::cluster_sync();
+#pragma unroll
+            for (int j = 0; j < NS / 2; ++j) h[j] = 0;
+            const uint32_t e = (uint32_t)__cvta_generic_to_shared(block);
+            for (int q = 0; q < rank; ++q) fold([&](int k) { return nb::ld_cluster(e + k * 128, q); });
+        } else {
+#pragma unroll
+            for (int j = 0; j < NS / 2; ++j) h[j] = 0;
+        }
+        fold_warps(warp - warp % a.tw, warp);
+        if (chunk == 0 && a.state_in) load_states(a.state_in + at, h);
+        pass(std::true_type{});
+        if (a.ranks > 1) nb::cluster_sync();  // no block leaves while another reads its shared memory
     } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (n0 + j < a.N) {
-                A2[j] = a.A[(int64_t)dd * a.N + n0 + j];
-                if (a.state_in) h[j] = a.state_in[sat + j];
-            }
+        pass(std::true_type{});
     }
+    if (a.state_out && on && chunk == chunks - 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) A2[j] *= LOG2E;
-    const float bias = a.dt_bias ? a.dt_bias[dd] : 0.0f, skip = a.skip ? a.skip[dd] : 0.0f;
-    const T *x = (const T *)a.x + s * a.x_ss + dd, *dt = (const T *)a.dt + s * a.dt_ss + dd;
-    const T *z = a.z ? (const T *)a.z + s * a.z_ss + dd : nullptr;
-    const int64_t bc = s * a.bc_ss + (int64_t)(dd / a.per_group) * a.N + n0;
-    const T *B = (const T *)a.B + bc, *C = (const T *)a.C + bc;
-    T *y = (T *)a.y + s * a.y_ss + dd;
-    for (int t = 0; t < len; ++t) {
-        float b[4], c[4];
+        for (int j = 0; j < NS / 2; j += 2) {
+            float f[4];
+            unpack2(h[j], f[0], f[1]);
+            unpack2(h[j + 1], f[2], f[3]);
+            float *p = a.state_out + at + 2 * j;
+            if (V4) {
+                if (n0 + 2 * j < a.N) *(float4 *)p = make_float4(f[0], f[1], f[2], f[3]);
+            } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = c[j] = 0.0f;
-        if (V4) {
-            if (n0 < a.N) {
-                const nb::Vec<T, 4> tb = *(const nb::Vec<T, 4> *)(B + (int64_t)t * a.bc_ld), tc = *(const nb::Vec<T, 4> *)(C + (int64_t)t * a.bc_ld);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { b[j] = nb::to_f32(tb.v[j]); c[j] = nb::to_f32(tc.v[j]); }
+                for (int k = 0; k < 4; ++k)
+                    if (n0 + 2 * j + k < a.N) p[k] = f[k];
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n0 + j < a.N) { b[j] = nb::to_f32(B[(int64_t)t * a.bc_ld + j]); c[j] = nb::to_f32(C[(int64_t)t * a.bc_ld + j]); }
-        }
-        const float xv = nb::to_f32(x[(int64_t)t * a.x_ld]);
-        float step = nb::to_f32(dt[(int64_t)t * a.dt_ld]) + bias;
-        if (a.softplus) step = softplus_f(step);
-        const float sx = step * xv;
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            h[j] = fmaf(exp2f(step * A2[j]), h[j], sx * b[j]);
-            sum = fmaf(h[j], c[j], sum);
-        }
-#pragma unroll
-        for (int o = LPC / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (on && lane % LPC == 0) {
-            float v = fmaf(skip, xv, sum);
-            if (z) {
-                const float zv = nb::to_f32(z[(int64_t)t * a.z_ld]);
-                v *= zv * nb::sigmoid_fast(zv);
-            }
-            y[(int64_t)t * a.y_ld] = nb::from_f32<T>(v);
-        }
-    }
-    if (a.state_out && on) {
-        if (V4) {
-            if (n0 < a.N) *(float4 *)(a.state_out + sat) = make_float4(h[0], h[1], h[2], h[3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n0 + j < a.N) a.state_out[sat + j] = h[j];
         }
     }
 }
 
-template <typename T, int LPC, bool V4>
-int run(ScanArgs a, cudaStream_t st) {
-    a.wps = (a.D * LPC + 31) / 32;
-    a.warps = (int64_t)a.streams * a.wps;
-    const int64_t blocks = (a.warps * 32 + NT - 1) / NT;
+template <typename T, int LPC, int NS, bool V4>
+int run_long(ScanArgs a, cudaStream_t st) {
+    constexpr int CPW = 32 / LPC, U = tile_rows<LPC>();
+    a.tiles = (a.per_group + CPW - 1) / CPW;
+    a.units = a.D / a.per_group * a.tiles;
+    a.items = (int64_t)a.streams * a.units;
+    // chunks of time until the warps fill the GPU, of at least four tiles each
+    int chunks = 1;
+    const int want = nb_scan_want();
+    if (a.items < nb_scan_split())
+        while (chunks < 64 && a.items * chunks < want && chunks * 2 * 32 <= a.c) chunks *= 2;
+    a.tw = chunks < LW ? chunks : LW;
+    a.ranks = chunks / a.tw;
+    const int per_block = LW / a.tw;
+    const int64_t blocks = (a.items + per_block - 1) / per_block * a.ranks;
     if (blocks > 0x7fffffff) return nb_set_error("nemo_selective_scan: too many streams");
-    nb::launch(selective_scan_kernel<T, LPC, V4>, dim3((unsigned)blocks), NT, 0, st, a);
-    return nb_check_launch("selective_scan_kernel");
+    const size_t smem = (LW * 2 * U * LPC * NS + (chunks > 1 ? (LW + 1) * (NS + 1) * 32 : 0)) * sizeof(float);
+    auto kernel = scan_long_kernel<T, LPC, NS, V4>;
+    if (nb_smem_attr((const void *)kernel, smem)) return -1;
+    if (a.ranks == 1) {
+        nb::launch(kernel, dim3((unsigned)blocks), 32 * LW, smem, st, a);
+    } else {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)blocks);
+        cfg.blockDim = dim3(32 * LW);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = a.ranks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = nb_pdl_enabled() ? 2 : 1;
+        cudaLaunchKernelEx(&cfg, kernel, a);
+    }
+    return nb_check_launch("scan_long_kernel");
 }
 
 template <typename T, bool V4>
-int by_states(const ScanArgs &a, cudaStream_t st) {
-    if (a.N <= 4) return run<T, 1, V4>(a, st);
-    if (a.N <= 8) return run<T, 2, V4>(a, st);
-    if (a.N <= 16) return run<T, 4, V4>(a, st);
-    if (a.N <= 32) return run<T, 8, V4>(a, st);
-    if (a.N <= 64) return run<T, 16, V4>(a, st);
-    return run<T, 32, V4>(a, st);
+int by_size(const ScanArgs &a, cudaStream_t st) {
+    if (a.c <= 16) {
+        if (a.N <= 4) return run_few<T, 1, V4>(a, st);
+        if (a.N <= 8) return run_few<T, 2, V4>(a, st);
+        if (a.N <= 16) return run_few<T, 4, V4>(a, st);
+        if (a.N <= 32) return run_few<T, 8, V4>(a, st);
+        if (a.N <= 64) return run_few<T, 16, V4>(a, st);
+        return run_few<T, 32, V4>(a, st);
+    }
+    if (a.N <= 4) return run_long<T, 1, 4, V4>(a, st);
+    if (a.N <= 8) return run_long<T, 1, 8, V4>(a, st);
+    if (a.N <= 16) return run_long<T, 1, 16, V4>(a, st);
+    if (a.N <= 32) return run_long<T, 2, 16, V4>(a, st);
+    if (a.N <= 64) return run_long<T, 4, 16, V4>(a, st);
+    return run_long<T, 8, 16, V4>(a, st);
 }
 
 }  // namespace
@@ -164,6 +603,6 @@ extern "C" int nemo_selective_scan(const nemo_selective_scan_args_t *p, void *st
                     (((uintptr_t)p->B | (uintptr_t)p->C) % (4 * es)) == 0 && ((p->bc_ld | p->bc_sstride) & 3) == 0;
     int rc = 0;
     cudaStream_t st = (cudaStream_t)stream;
-    NB_ELT_SWITCH(p->elt, T, rc = v4 ? by_states<T, true>(a, st) : by_states<T, false>(a, st));
+    NB_ELT_SWITCH(p->elt, T, rc = v4 ? by_size<T, true>(a, st) : by_size<T, false>(a, st));
     return rc;
 }

@@ -256,6 +256,18 @@ __device__ __forceinline__ f2 softplus2(f2 v) {
 // before it, h <- exp(A sum of steps) h + end, and the chunks run again from it, writing y. Nothing
 // but shared memory is needed for that, and the order of the sums is fixed.
 constexpr int LW = 8;  // warps per block
+// An element as it is loaded, and its value: kept apart, so that nothing waits for a load until its
+// value is used
+__device__ __forceinline__ uint32_t raw(const float *p) { return __float_as_uint(*p); }
+__device__ __forceinline__ uint32_t raw(const __nv_bfloat16 *p) { return *(const unsigned short *)p; }
+__device__ __forceinline__ uint32_t raw(const __half *p) { return *(const unsigned short *)p; }
+template <typename T>
+__device__ __forceinline__ float cooked(uint32_t v) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(v);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(v << 16);
+    else return __half2float(__ushort_as_half((unsigned short)v));
+}
+
 template <int LPC>
 constexpr int tile_rows() { return LPC < 4 ? 4 : LPC; }  // at least one row per lane of a channel
 
@@ -313,7 +325,7 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
     auto pass = [&](auto write) __attribute__((always_inline)) {
         constexpr bool WRITE = decltype(write)::value;
         float total = 0.0f;
-        T rx[RP], rd[RP], rz[RP];
+        uint32_t rx[RP], rd[RP], rz[RP];
         nb::Vec<T, 4> rb[QL], rc[QL];
         // this lane's next rows of x, dt, z and its groups of B and C
         const T *px = X + (int64_t)(tb + sub * RP) * a.x_ld, *pd = DT + (int64_t)(tb + sub * RP) * a.dt_ld;
@@ -325,11 +337,10 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
             const bool all = left >= U;
 #pragma unroll
             for (int r = 0; r < RP; ++r) {
-                if (all || sub * RP + r < left) {
-                    rx[r] = px[r * a.x_ld];
-                    rd[r] = pd[r * a.dt_ld];
-                    if (WRITE && Z) rz[r] = pz[r * a.z_ld];
-                }
+                const int k = all ? r : min(sub * RP + r, left - 1) - sub * RP;  // a row that does not exist: the last one
+                rx[r] = raw(px + k * a.x_ld);
+                rd[r] = raw(pd + k * a.dt_ld);
+                if (WRITE && Z) rz[r] = raw(pz + k * a.z_ld);
             }
             px += U * a.x_ld;
             pd += U * a.dt_ld;
@@ -376,9 +387,9 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
             float xv[RP], step[RP], sx[RP], gate[RP];
 #pragma unroll
             for (int r = 0; r < RP; ++r) {
-                xv[r] = nb::to_f32(rx[r]);
-                step[r] = nb::to_f32(rd[r]) + bias;
-                if (WRITE && Z) gate[r] = nb::to_f32(rz[r]);
+                xv[r] = cooked<T>(rx[r]);
+                step[r] = cooked<T>(rd[r]) + bias;
+                if (WRITE && Z) gate[r] = cooked<T>(rz[r]);
             }
             const int live = te - t0;  // rows of this tile that exist
             if (live > U) fetch(live - U);

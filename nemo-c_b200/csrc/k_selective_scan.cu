@@ -2,24 +2,16 @@
 //
 //   h[d][n] = exp(step A[d][n]) h[d][n] + step x[d] B[n],   y[d] = (sum_n h[d][n] C[n] + skip[d] x[d]) silu(z[d])
 //
-// The state is held in fp32 registers: LPC lanes share a channel, NS states each, so that a warp
-// reads the state of its channels as one contiguous run. What belongs to a (row, channel) and not to
-// a state (the step with its softplus, the gate, the output) is computed once, by one lane for the
-// others, and the sums over the states of V rows are folded together: V values over LPC lanes take
-// about V shuffles, and each row's sum ends in the lane that writes it.
+// The state is held in fp32 registers. What belongs to a (row, channel) and not to a state (the step with
+// its softplus, the gate, the output) is computed once. Where LPC lanes share a channel, rows (or
+// streams) are dealt out among them for that, and the sums over the states of several rows are folded
+// together: V values over LPC lanes take about V shuffles, and each sum ends in the lane that writes it.
 //
-// Two kernels. Few rows: the state's bytes (8 N per channel) dominate, the kernel is bound by HBM;
-// warps load everything of their rows at once and nothing is staged. Many rows: bound by the
-// exponentials (one per row, channel and state on the special-function units, 16 a clock an SM); half
-// of a block's warps prepare tiles of rows in shared memory and write the finished ones out while
-// the other half runs the recurrence.
+// Two kernels: single rows, bound by the state's bytes, and runs of rows, bound by the exponentials
+// (one per row, channel and state on the special-function units, 16 a clock an SM).
 #include <type_traits>
-#include <cstdlib>
 #include "elt.cuh"
 #include "cluster.cuh"
-
-static int nb_scan_want() { const char *e = getenv("WANT"); return e ? atoi(e) : 148 * 32; }
-static int nb_scan_split() { const char *e = getenv("SPLIT"); return e ? atoi(e) : 148 * 5; }
 
 namespace {
 
@@ -35,8 +27,8 @@ struct ScanArgs {
     const int *lens;
     int streams, c, D, N, per_group, softplus;
     int tiles, units;  // a warp's worth of channels: of a group, of a stream
-    int64_t items;     // few rows: warps; many rows: channel tiles of all streams
-    int tw, ranks;     // many rows: chunks of time in a block, blocks of a cluster
+    int64_t items;     // single rows: warps; runs: channel tiles of all streams
+    int tw, ranks;     // runs: chunks of time in a block, blocks of a cluster
 };
 
 __device__ __forceinline__ float ex2(float v) {
@@ -60,27 +52,28 @@ __device__ __forceinline__ float softplus_f(float v) {
     return fmaf(2.0f, p, fmaxf(v, 0.0f));
 }
 
-// ---- few rows --------------------------------------------------------------------------------
-// A warp owns 32 / LPC channels. STEP (one row per stream): V streams at a time, their rows taken
-// together, so that V states are in flight per channel and A is read once for them. Otherwise: one
-// stream, V rows at a time.
-constexpr int FEW_NT = 128;
+// ---- single rows -----------------------------------------------------------------------------
+// One row per stream: bound by HBM (8 N bytes of state per channel). A warp owns 32 / LPC channels of
+// SB streams: the streams' rows are taken together, so that SB states are in flight per lane and A is
+// read once for them.
+constexpr int STEP_NT = 128, STEP_SB = 4;
 
-template <typename T, int LPC, bool V4, bool STEP>
-__global__ void __launch_bounds__(FEW_NT) scan_few_kernel(const __grid_constant__ ScanArgs a) {
-    constexpr int CPW = 32 / LPC, V = LPC < 4 ? LPC : 4, REP = LPC / V;
+template <typename T, int LPC, bool V4>
+__global__ void __launch_bounds__(STEP_NT, 6) scan_step_kernel(const __grid_constant__ ScanArgs a) {
+    constexpr int CPW = 32 / LPC, SB = LPC < STEP_SB ? LPC : STEP_SB, REP = LPC / SB;
     nb::pdl_wait();
-    const int64_t w = ((int64_t)blockIdx.x * FEW_NT + threadIdx.x) >> 5;
+    const int64_t w = ((int64_t)blockIdx.x * STEP_NT + threadIdx.x) >> 5;
     if (w >= a.items) return;
-    const int lane = threadIdx.x & 31, sub = lane % LPC, n0 = sub * 4, v = sub / REP;  // this lane's states, and its row of V
-    const int64_t sblk = w / a.units;
-    const int unit = (int)(w - sblk * a.units), grp = unit / a.tiles;
+    const int lane = threadIdx.x & 31, sub = lane % LPC, n0 = sub * 4, v = sub / REP;  // this lane's states, and its stream of SB
+    const int64_t s0 = w / a.units * SB;
+    const int unit = (int)(w % a.units), grp = unit / a.tiles;
     const int dg = (unit - grp * a.tiles) * CPW + lane / LPC;
-    const bool on = dg < a.per_group;
+    const bool on = dg < a.per_group, st4 = n0 < a.N;
     const int d = grp * a.per_group + (on ? dg : a.per_group - 1);
-    const bool st4 = n0 < a.N;
 
-    auto load4 = [&](const float *p, float (&o)[4]) {
+    auto load4 = [&](const float *p, float (&o)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = 0.0f;
         if (V4) {
             if (st4) {
                 const float4 t = *(const float4 *)p;
@@ -92,7 +85,9 @@ __global__ void __launch_bounds__(FEW_NT) scan_few_kernel(const __grid_constant_
                 if (n0 + j < a.N) o[j] = p[j];
         }
     };
-    auto loadbc = [&](const T *p, float (&o)[4]) {
+    auto load4t = [&](const T *p, float (&o)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = 0.0f;
         if (V4) {
             if (st4) {
                 const nb::Vec<T, 4> t = *(const nb::Vec<T, 4> *)p;
@@ -105,99 +100,84 @@ __global__ void __launch_bounds__(FEW_NT) scan_few_kernel(const __grid_constant_
                 if (n0 + j < a.N) o[j] = nb::to_f32(p[j]);
         }
     };
-    auto store4 = [&](float *p, const float (&o)[4]) {
-        if (V4) {
-            if (st4) *(float4 *)p = make_float4(o[0], o[1], o[2], o[3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n0 + j < a.N) p[j] = o[j];
-        }
-    };
 
-    const int64_t s0 = STEP ? sblk * V : sblk;
-    constexpr int H = STEP ? V : 1;
-    float h[H][4], A2[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+    float h[SB][4], A2[4], b[SB][4], c[SB][4];
+    const int64_t at = (s0 * a.D + d) * (int64_t)a.N + n0, per_stream = (int64_t)a.D * a.N;
 #pragma unroll
-    for (int r = 0; r < H; ++r) {
+    for (int r = 0; r < SB; ++r) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) h[r][j] = 0.0f;
-        if (a.state_in && s0 + r < a.streams) load4(a.state_in + ((s0 + r) * a.D + d) * (int64_t)a.N + n0, h[r]);
+        if (a.state_in && s0 + r < a.streams) load4(a.state_in + at + r * per_stream, h[r]);
+    }
+    const int64_t s = s0 + v;  // this lane's stream: it computes the stream's step and writes its output
+    const bool live = s < a.streams && (!a.lens || a.lens[s] > 0);
+    float xv = 0.0f, step = 0.0f, gate = 1.0f;
+    if (s < a.streams) {  // not after lens: a row that is not its stream's may be read, not used
+        xv = nb::to_f32(((const T *)a.x)[s * a.x_ss + d]);
+        step = nb::to_f32(((const T *)a.dt)[s * a.dt_ss + d]);
+        if (a.z) gate = nb::to_f32(((const T *)a.z)[s * a.z_ss + d]);
     }
     load4(a.A + (int64_t)d * a.N + n0, A2);
-    const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, skip = a.skip ? a.skip[d] : 0.0f;
-    const int64_t bc0 = (int64_t)grp * a.N + n0;
-    const int len = STEP ? 1 : a.lens ? max(0, min(a.lens[s0], a.c)) : a.c;
-
-    for (int t0 = 0; t0 < len; t0 += V) {
-        // this lane's row: of stream s0 + v (STEP), or row t0 + v
-        const int64_t s = STEP ? s0 + v : s0;
-        const int t = STEP ? 0 : t0 + v;
-        const bool live = STEP ? s < a.streams && (!a.lens || a.lens[s] > 0) : t < len;
-        float xv = 0.0f, step = 0.0f, gate = 1.0f;
-        if (live) {
-            xv = nb::to_f32(((const T *)a.x)[s * a.x_ss + t * a.x_ld + d]);
-            step = nb::to_f32(((const T *)a.dt)[s * a.dt_ss + t * a.dt_ld + d]);
-            if (a.z) gate = nb::to_f32(((const T *)a.z)[s * a.z_ss + t * a.z_ld + d]);
-        }
-        float b[V][4], c[V][4];
+    const int64_t bc0 = s0 * a.bc_ss + (int64_t)grp * a.N + n0;
 #pragma unroll
-        for (int r = 0; r < V; ++r) {
+    for (int r = 0; r < SB; ++r) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[r][j] = c[r][j] = 0.0f;
-            const int64_t at = STEP ? (s0 + r) * a.bc_ss + bc0 : s0 * a.bc_ss + (t0 + r) * a.bc_ld + bc0;
-            if (STEP ? s0 + r < a.streams : t0 + r < len) {
-                loadbc((const T *)a.B + at, b[r]);
-                loadbc((const T *)a.C + at, c[r]);
-            }
-        }
-        if (live) {
-            step += bias;
-            if (a.softplus) step = softplus_f(step);
-            if (a.z) gate *= nb::sigmoid_fast(gate);
-        }
-        const float sx = step * xv;
-        float sum[V];
-#pragma unroll
-        for (int r = 0; r < V; ++r) {
-            const float sr = __shfl_sync(0xffffffffu, step, r * REP, LPC) * LOG2E, xr = __shfl_sync(0xffffffffu, sx, r * REP, LPC);
-            const bool go = STEP ? __shfl_sync(0xffffffffu, (int)live, r * REP, LPC) != 0 : t0 + r < len;
-            sum[r] = 0.0f;
-            if (go) {
-                float (&hh)[4] = h[STEP ? r : 0];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    hh[j] = fmaf(ex2(sr * A2[j]), hh[j], xr * b[r][j]);
-                    sum[r] = fmaf(hh[j], c[r][j], sum[r]);
-                }
-            }
-        }
-        nb::WarpFold<V, LPC / 2>::run(sum, lane);
-        if (live && on && sub % REP == 0) {
-            const float o = fmaf(skip, xv, sum[0]) * gate;
-            ((T *)a.y)[s * a.y_ss + t * a.y_ld + d] = nb::from_f32<T>(o);
+        for (int j = 0; j < 4; ++j) b[r][j] = c[r][j] = 0.0f;
+        if (s0 + r < a.streams) {
+            load4t((const T *)a.B + bc0 + r * a.bc_ss, b[r]);
+            load4t((const T *)a.C + bc0 + r * a.bc_ss, c[r]);
         }
     }
+    if (live) {
+        step += a.dt_bias ? a.dt_bias[d] : 0.0f;
+        if (a.softplus) step = softplus_f(step);
+        if (a.z) gate *= nb::sigmoid_fast(gate);
+    }
+    const float sx = step * xv;
+    float sum[SB];
+#pragma unroll
+    for (int r = 0; r < SB; ++r) {
+        const float sr = __shfl_sync(0xffffffffu, step, r * REP, LPC) * LOG2E, xr = __shfl_sync(0xffffffffu, sx, r * REP, LPC);
+        sum[r] = 0.0f;
+        if (__shfl_sync(0xffffffffu, (int)live, r * REP, LPC)) {  // the same for the whole warp; without a row the state stays
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h[r][j] = fmaf(ex2(sr * A2[j]), h[r][j], xr * b[r][j]);
+                sum[r] = fmaf(h[r][j], c[r][j], sum[r]);
+            }
+        }
+    }
+    nb::WarpFold<SB, LPC / 2>::run(sum, lane);
+    if (live && on && sub % REP == 0)
+        ((T *)a.y)[s * a.y_ss + d] = nb::from_f32<T>(fmaf(a.skip ? a.skip[d] : 0.0f, xv, sum[0]) * gate);
     if (a.state_out && on)
 #pragma unroll
-        for (int r = 0; r < H; ++r)
-            if (s0 + r < a.streams) store4(a.state_out + ((s0 + r) * a.D + d) * (int64_t)a.N + n0, h[r]);
+        for (int r = 0; r < SB; ++r)
+            if (s0 + r < a.streams) {
+                float *p = a.state_out + at + r * per_stream;
+                if (V4) {
+                    if (st4) *(float4 *)p = make_float4(h[r][0], h[r][1], h[r][2], h[r][3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (n0 + j < a.N) p[j] = h[r][j];
+                }
+            }
 }
 
 template <typename T, int LPC, bool V4>
-int run_few(ScanArgs a, cudaStream_t st) {
-    constexpr int CPW = 32 / LPC, V = LPC < 4 ? LPC : 4;
+int run_step(ScanArgs a, cudaStream_t st) {
+    constexpr int CPW = 32 / LPC, SB = LPC < STEP_SB ? LPC : STEP_SB;
     a.tiles = (a.per_group + CPW - 1) / CPW;
     a.units = a.D / a.per_group * a.tiles;
-    const bool step = a.c == 1;
-    a.items = (step ? (a.streams + V - 1) / V : a.streams) * (int64_t)a.units;
-    const int64_t blocks = (a.items * 32 + FEW_NT - 1) / FEW_NT;
+    a.items = (a.streams + SB - 1) / SB * (int64_t)a.units;
+    const int64_t blocks = (a.items * 32 + STEP_NT - 1) / STEP_NT;
     if (blocks > 0x7fffffff) return nb_set_error("nemo_selective_scan: too many streams");
-    nb::launch(step ? scan_few_kernel<T, LPC, V4, true> : scan_few_kernel<T, LPC, V4, false>, dim3((unsigned)blocks), FEW_NT, 0, st, a);
-    return nb_check_launch("scan_few_kernel");
+    nb::launch(scan_step_kernel<T, LPC, V4>, dim3((unsigned)blocks), STEP_NT, 0, st, a);
+    return nb_check_launch("scan_step_kernel");
 }
 
-// ---- many rows -------------------------------------------------------------------------------
+// ---- runs of rows ----------------------------------------------------------------------------
 
 typedef unsigned long long f2;  // two fp32 in a register pair
 __device__ __forceinline__ f2 pack2(float lo, float hi) {
@@ -533,11 +513,14 @@ int run_long(ScanArgs a, cudaStream_t st) {
     a.tiles = (a.per_group + CPW - 1) / CPW;
     a.units = a.D / a.per_group * a.tiles;
     a.items = (int64_t)a.streams * a.units;
-    // chunks of time until the warps fill the GPU, of at least four tiles each
+    // Time is cut where the channels give less than five warps an SM: a chunk costs its rows twice, less
+    // the outputs (16384 rows of 2048 channels: 10.6 ms whole, 0.50 ms in 64 chunks; 24 streams of 600 rows
+    // of 1024 channels, 5.2 warps an SM: 0.22 ms whole, 0.21 to 0.25 ms in 2 to 8). Then until there are
+    // 32 warps an SM (8 streams of up to 2500 rows of 2048 channels: 0.62 ms with 8, 0.40 ms with 16, 0.35 ms with
+    // 32), at 32 rows a chunk at least.
     int chunks = 1;
-    const int want = nb_scan_want();
-    if (a.items < nb_scan_split())
-        while (chunks < 64 && a.items * chunks < want && chunks * 2 * 32 <= a.c) chunks *= 2;
+    if (a.items < 148 * 5)
+        while (chunks < 64 && a.items * chunks < 148 * 32 && chunks * 2 * 32 <= a.c) chunks *= 2;
     a.tw = chunks < LW ? chunks : LW;
     a.ranks = chunks / a.tw;
     const int per_block = LW / a.tw;
@@ -569,13 +552,14 @@ int run_long(ScanArgs a, cudaStream_t st) {
 
 template <typename T, bool V4>
 int by_size(const ScanArgs &a, cudaStream_t st) {
-    if (a.c <= 16) {
-        if (a.N <= 4) return run_few<T, 1, V4>(a, st);
-        if (a.N <= 8) return run_few<T, 2, V4>(a, st);
-        if (a.N <= 16) return run_few<T, 4, V4>(a, st);
-        if (a.N <= 32) return run_few<T, 8, V4>(a, st);
-        if (a.N <= 64) return run_few<T, 16, V4>(a, st);
-        return run_few<T, 32, V4>(a, st);
+    // (runs of 2 rows for 256 streams of 2048 channels: 30 us with the kernel for runs, 61 us row by row)
+    if (a.c == 1) {
+        if (a.N <= 4) return run_step<T, 1, V4>(a, st);
+        if (a.N <= 8) return run_step<T, 2, V4>(a, st);
+        if (a.N <= 16) return run_step<T, 4, V4>(a, st);
+        if (a.N <= 32) return run_step<T, 8, V4>(a, st);
+        if (a.N <= 64) return run_step<T, 16, V4>(a, st);
+        return run_step<T, 32, V4>(a, st);
     }
     if (a.N <= 4) return run_long<T, 1, 4, V4>(a, st);
     if (a.N <= 8) return run_long<T, 1, 8, V4>(a, st);

@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace nb {
 
@@ -27,15 +28,6 @@ struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Vec {
 
 inline int elt_size(int elt) { return elt == NEMO_ELT_F32 ? 4 : 2; }
 inline bool elt_ok(int elt) { return elt == NEMO_ELT_F32 || elt == NEMO_ELT_BF16 || elt == NEMO_ELT_F16; }
-
-// 1 / (1 + e^-v) on the special-function units (a few ulp of fp32; an infinite exponential gives 0,
-// a NaN stays one)
-__device__ __forceinline__ float sigmoid_fast(float v) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    return r;
-}
 
 }  // namespace nb
 

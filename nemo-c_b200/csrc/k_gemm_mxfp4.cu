@@ -23,6 +23,7 @@
 // error, takes part in the remaining cluster barriers and unwinds.
 #include <cuda.h>
 #include <cstring>
+#include <cstdlib>
 #include <atomic>
 #include "cluster.cuh"
 #include "elt.cuh"
@@ -96,6 +97,33 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uin
         : "memory");
 }
 
+// 32 lanes x CN consecutive columns; the values are there after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+          "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+        "%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+          "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]),
+          "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+// Waits for this warp's loads; naming the loaded values keeps their uses behind the wait.
+template <int CN>
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[CN]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < CN; ++j) asm volatile("" : "+f"(v[j]));
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
 }
@@ -113,6 +141,45 @@ __device__ __forceinline__ void finish(const MxArgs &p, int m, int n, float va, 
     T *c = (T *)p.C + (int64_t)m * p.ldc + n;
     if (p.accumulate) v += nb::to_f32(*c);
     *c = nb::from_f32<T>(v);
+}
+// The same for CN rows of one output column, in pairs; v holds the accumulators, g GLU's gates.
+template <int ACT, int CN>
+__device__ __forceinline__ void activate(float (&v)[CN], const float (&g)[CN], float ba, float bb, float alpha) {
+#pragma unroll
+    for (int j = 0; j < CN; j += 2) {
+        nb::f2 x = nb::add2(nb::pack2(v[j], v[j + 1]), nb::dup2(ba));
+        if (ACT == NEMO_ACT_SILU) x = nb::mul2(x, nb::sigmoid2(x));
+        if (ACT == NEMO_ACT_GLU) x = nb::mul2(x, nb::sigmoid2(nb::add2(nb::pack2(g[j], g[j + 1]), nb::dup2(bb))));
+        if (ACT == NEMO_ACT_RELU) {
+            float a, b;
+            nb::unpack2(x, a, b);
+            x = nb::pack2(a < 0.0f ? 0.0f : a, b < 0.0f ? 0.0f : b);
+        }
+        nb::unpack2(nb::mul2(x, nb::dup2(alpha)), v[j], v[j + 1]);
+    }
+}
+template <typename T, int CN>
+__device__ __forceinline__ void finish_rows(const MxArgs &p, int m, int n, int count, float (&v)[CN], const float (&g)[CN], float ba, float bb) {
+    switch (p.act) {
+        case NEMO_ACT_SILU: activate<NEMO_ACT_SILU, CN>(v, g, ba, bb, p.alpha); break;
+        case NEMO_ACT_RELU: activate<NEMO_ACT_RELU, CN>(v, g, ba, bb, p.alpha); break;
+        case NEMO_ACT_GLU: activate<NEMO_ACT_GLU, CN>(v, g, ba, bb, p.alpha); break;
+        default: activate<NEMO_ACT_NONE, CN>(v, g, ba, bb, p.alpha); break;
+    }
+    T *c = (T *)p.C + (int64_t)m * p.ldc + n;
+    if (p.accumulate) {
+#pragma unroll
+        for (int j = 0; j < CN; ++j)
+            if (j < count) v[j] += nb::to_f32(c[j * p.ldc]);
+    }
+    if (count >= CN) {
+#pragma unroll
+        for (int j = 0; j < CN; ++j, c += p.ldc) *c = nb::from_f32<T>(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < CN; ++j, c += p.ldc)
+            if (j < count) *c = nb::from_f32<T>(v[j]);
+    }
 }
 
 template <typename T, int BN, int WT>
@@ -256,14 +323,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const bool on = n < nout;
                     const float ba = on && p.bias ? p.bias[n] : 0.0f, bb = on && glu && p.bias ? p.bias[n + p.N / 2] : 0.0f;
                     const uint32_t acc = lanes + ((t * WT + i) % C::SLOTS) * BN, gate = lanes + ((t * WT + 1) % C::SLOTS) * BN;
-                    for (int j0 = jbeg; j0 < jend && j0 < mcount; j0 += 16) {
-                        float v[16], g[16];
-                        sm100::tmem_ld16(acc + j0, v);
-                        if (WT == 2 && glu) sm100::tmem_ld16(gate + j0, g);
-                        if (on)
-#pragma unroll
-                            for (int jj = 0; jj < 16; ++jj)
-                                if (j0 + jj < mcount) finish<T>(p, m0 + j0 + jj, n, v[jj], WT == 2 ? g[jj] : 0.0f, ba, bb);
+                    constexpr int CN = BN >= 64 && WT == 1 ? 32 : 16;  // columns per load
+                    for (int j0 = jbeg; j0 < jend && j0 < mcount; j0 += CN) {
+                        float v[CN], g[CN];
+                        tmem_ld(acc + j0, v);
+                        if (WT == 2 && glu) tmem_ld(gate + j0, g);
+                        tmem_wait_ld(v);
+                        if (WT == 2 && glu) tmem_wait_ld(g);
+                        if (on) finish_rows<T, CN>(p, m0 + j0, n, mcount - j0, v, g, ba, bb);
                     }
                 }
                 sm100::tc_fence_before();
@@ -391,6 +458,15 @@ int run(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
 template <typename T>
 int by_rows(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
     const bool glu = a->act == NEMO_ACT_GLU;
+    const char *e = getenv("MXCFG");
+    if (e) {
+        int bn = atoi(e), wt = atoi(strchr(e, ',') + 1);
+        if (glu) wt = 2;
+        if (bn == 16 && a->M <= 16) return wt == 1 ? run<T, 16, 1>(a, st) : run<T, 16, 2>(a, st);
+        if (bn == 32 && a->M <= 32) return wt == 1 ? run<T, 32, 1>(a, st) : run<T, 32, 2>(a, st);
+        if (bn == 64 && a->M <= 64) return wt == 1 ? run<T, 64, 1>(a, st) : run<T, 64, 2>(a, st);
+        if (bn == 128) return wt == 1 ? run<T, 128, 1>(a, st) : run<T, 128, 2>(a, st);
+    }
     if (a->M <= 16) return glu ? run<T, 16, 2>(a, st) : run<T, 16, 1>(a, st);
     if (a->M <= 64) return glu ? run<T, 64, 2>(a, st) : run<T, 64, 1>(a, st);
     return glu ? run<T, 128, 2>(a, st) : run<T, 128, 1>(a, st);

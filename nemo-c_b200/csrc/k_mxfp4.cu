@@ -8,7 +8,7 @@
 // A block that holds an infinity or a NaN has no such scale: its byte is 255 (the format's NaN)
 // and its codes are zero, so every value of it reads back as NaN.
 //
-// Both kernels are bound by HBM (2.03 to 6.03 bytes moved per element and no reuse).
+// Both kernels are bound by HBM (2.5 to 4.5 bytes moved per element, no reuse).
 #include "elt.cuh"
 #include "mxfp4.cuh"
 
@@ -30,107 +30,113 @@ __device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
     return r;
 }
 
-// Four neighbouring lanes share a block, eight columns each. Lanes of a warp past the last column
-// group still take part in the exchange.
-template <typename T, bool VEC>
+// (row, column group) of group i of a row-major sequence with `per` groups a row
+__device__ __forceinline__ void place(int64_t i, int64_t total, int per, int64_t &row, int &g) {
+    if (total <= 0xffffffffLL) {
+        const uint32_t r = (uint32_t)i / (uint32_t)per;
+        row = r;
+        g = (int)((uint32_t)i - r * (uint32_t)per);
+    } else {
+        row = i / per;
+        g = (int)(i - row * per);
+    }
+}
+
+// Two neighbouring lanes share a block, 16 columns each (32 or 64 bytes in flight a lane). TILES: K is a
+// multiple of 128, so eight lanes always hold a row's four blocks of one scale tile, whose bytes are
+// stored as one word. Lanes past the last group still take part in the exchange.
+template <typename T, bool VEC, bool TILES>
 __global__ void __launch_bounds__(NT) mxfp4_quantize_kernel(const T *X, int64_t ldx, int64_t groups, int gpr, uint8_t *Q, int64_t ldq, uint8_t *S) {
     nb::pdl_wait();
-    const int kt = (gpr + 15) / 16;  // scale tiles along a row
-    const int64_t step = (int64_t)gridDim.x * NT;
-    for (int64_t i0 = (int64_t)blockIdx.x * NT; i0 < groups; i0 += step) {
-        const int64_t i = i0 + threadIdx.x;
-        const bool live = i < groups;
-        const int64_t ii = live ? i : groups - 1;
-        int64_t row;
-        int g;
-        if (groups <= 0xffffffffLL) {
-            const uint32_t r32 = (uint32_t)ii / (uint32_t)gpr;
-            row = r32;
-            g = (int)((uint32_t)ii - r32 * (uint32_t)gpr);
-        } else {
-            row = ii / gpr;
-            g = (int)(ii - row * gpr);
-        }
-        const T *x = X + row * ldx + (int64_t)g * 8;
-        float v[8];
-        if (VEC) {
-            constexpr int E = 16 / sizeof(T);
+    const int kt = (gpr + 7) / 8;  // scale tiles along a row
+    const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
+    const bool live = i < groups;
+    int64_t row;
+    int g;
+    place(live ? i : groups - 1, groups, gpr, row, g);
+    const T *x = X + row * ldx + (int64_t)g * 16;
+    float v[16];
+    if (VEC) {
+        constexpr int E = 16 / sizeof(T);
+        nb::Vec<T, E> t[16 / E];
 #pragma unroll
-            for (int j = 0; j < 8 / E; ++j) {
-                const nb::Vec<T, E> t = *(const nb::Vec<T, E> *)(x + j * E);
+        for (int j = 0; j < 16 / E; ++j) t[j] = ((const nb::Vec<T, E> *)x)[j];
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[j * E + e] = nb::to_f32(t.v[e]);
-            }
-        } else {
+        for (int j = 0; j < 16; ++j) v[j] = nb::to_f32(t[j / E].v[j % E]);
+    } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = nb::to_f32(x[j]);
-        }
-        uint32_t top = 0;  // magnitudes compare as their bits; infinities and NaN are the largest
+        for (int j = 0; j < 16; ++j) v[j] = nb::to_f32(x[j]);
+    }
+    uint32_t top = 0;  // magnitudes compare as their bits; infinities and NaN are the largest
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int ex = (int)(top >> 23);
-        const bool bad = ex == 255;
-        const int byte = bad ? 255 : max(ex - 2, 0);
-        const float inv = bad ? 0.0f : __uint_as_float((uint32_t)(254 - byte) << 23);  // 2^(127 - byte), byte <= 252
+    for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const int ex = (int)(top >> 23);
+    const bool bad = ex == 255;
+    const int byte = bad ? 255 : max(ex - 2, 0);
+    const float inv = bad ? 0.0f : __uint_as_float((uint32_t)(254 - byte) << 23);  // 2^(127 - byte), byte <= 252
+    uint32_t codes[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv;
-        uint32_t codes = pack8(v);
-        if (bad) codes = 0;
-        if (live) {
-            uint8_t *q = Q + row * ldq + (int64_t)g * 4;
-            if (VEC) {
-                *(uint32_t *)q = codes;
-            } else {
+    for (int k = 0; k < 2; ++k) {
+        float w[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) q[j] = (uint8_t)(codes >> (8 * j));
-            }
-            if ((g & 3) == 0) {
-                uint8_t *s = S + mxfp4::scale_at(row, g >> 2, kt);
-                *s = (uint8_t)byte;
-                if (g + 4 == gpr)  // the row's last block: the rest of its tile reads as 2^-127
-                    for (int p = (g >> 2) % 4 + 1, o = 1; p < 4; ++p, ++o) s[o] = 0;
-            }
-        }
+        for (int j = 0; j < 8; ++j) w[j] = v[8 * k + j] * inv;
+        codes[k] = bad ? 0u : pack8(w);
+    }
+    uint32_t word = (uint32_t)byte;
+    if (TILES) {  // lane 8 m gathers the bytes of its own, the next, .. of four blocks
+        word |= __shfl_down_sync(0xffffffffu, word, 2) << 8;
+        word |= __shfl_down_sync(0xffffffffu, word, 4) << 16;
+    }
+    if (!live) return;
+    uint8_t *q = Q + row * ldq + (int64_t)g * 8;
+    if (VEC) {
+        *(uint2 *)q = make_uint2(codes[0], codes[1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = (uint8_t)(codes[j >> 2] >> (8 * (j & 3)));
+    }
+    if (TILES) {
+        if ((g & 7) == 0) *(uint32_t *)(S + mxfp4::scale_at(row, g >> 1, kt)) = word;
+    } else if ((g & 1) == 0) {
+        uint8_t *s = S + mxfp4::scale_at(row, g >> 1, kt);
+        *s = (uint8_t)byte;
+        if (g + 2 == gpr)  // the row's last block: the rest of its tile reads as 2^-127
+            for (int p = (g >> 1) % 4 + 1, o = 1; p < 4; ++p, ++o) s[o] = 0;
     }
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(NT) mxfp4_dequantize_kernel(const uint8_t *Q, int64_t ldq, const uint8_t *S, int64_t groups, int gpr, T *Y, int64_t ldy) {
     nb::pdl_wait();
-    const int kt = (gpr + 15) / 16;
-    const int64_t step = (int64_t)gridDim.x * NT;
-    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < groups; i += step) {
-        int64_t row;
-        int g;
-        if (groups <= 0xffffffffLL) {
-            const uint32_t r32 = (uint32_t)i / (uint32_t)gpr;
-            row = r32;
-            g = (int)((uint32_t)i - r32 * (uint32_t)gpr);
-        } else {
-            row = i / gpr;
-            g = (int)(i - row * gpr);
-        }
-        const uint8_t *q = Q + row * ldq + (int64_t)g * 4;
-        uint32_t codes;
-        if (VEC)
-            codes = *(const uint32_t *)q;
-        else
-            codes = q[0] | (uint32_t)q[1] << 8 | (uint32_t)q[2] << 16 | (uint32_t)q[3] << 24;
-        const float scale = mxfp4::scale_value(S[mxfp4::scale_at(row, g >> 2, kt)]);
-        T *y = Y + row * ldy + (int64_t)g * 8;
-        T o[8];
+    const int kt = (gpr + 7) / 8;
+    const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
+    if (i >= groups) return;
+    int64_t row;
+    int g;
+    place(i, groups, gpr, row, g);
+    const uint8_t *q = Q + row * ldq + (int64_t)g * 8;
+    uint32_t codes[2];
+    if (VEC) {
+        const uint2 t = *(const uint2 *)q;
+        codes[0] = t.x;
+        codes[1] = t.y;
+    } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = nb::from_f32<T>(mxfp4::code_value(codes >> (4 * j)) * scale);
-        if (VEC) {
-            constexpr int E = 16 / sizeof(T);
+        for (int k = 0; k < 2; ++k) codes[k] = q[4 * k] | (uint32_t)q[4 * k + 1] << 8 | (uint32_t)q[4 * k + 2] << 16 | (uint32_t)q[4 * k + 3] << 24;
+    }
+    const float scale = mxfp4::scale_value(S[mxfp4::scale_at(row, g >> 1, kt)]);
+    T *y = Y + row * ldy + (int64_t)g * 16;
+    constexpr int E = 16 / sizeof(T);
+    nb::Vec<T, E> o[16 / E];
 #pragma unroll
-            for (int j = 0; j < 8 / E; ++j) *(nb::Vec<T, E> *)(y + j * E) = *(const nb::Vec<T, E> *)(o + j * E);
-        } else {
+    for (int j = 0; j < 16; ++j) o[j / E].v[j % E] = nb::from_f32<T>(mxfp4::code_value(codes[j >> 3] >> (4 * (j & 7))) * scale);
+    if (VEC) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = o[j];
-        }
+        for (int j = 0; j < 16 / E; ++j) ((nb::Vec<T, E> *)y)[j] = o[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] = o[j / E].v[j % E];
     }
 }
 
@@ -154,13 +160,16 @@ extern "C" int64_t nemo_mxfp4_scale_bytes(int64_t rows, int64_t K) {
 extern "C" int nemo_mxfp4_quantize(const void *X, int x_elt, int64_t ldx, int64_t rows, int64_t K, uint8_t *codes, int64_t ldq, uint8_t *scales, void *stream) {
     if (check("nemo_mxfp4_quantize", X, x_elt, ldx, rows, K, codes, ldq, scales)) return -1;
     if (rows == 0 || K == 0) return 0;
-    const int64_t groups = rows * (K / 8);
-    const int64_t blocks = (groups + NT - 1) / NT;
-    const int grid = (int)(blocks < 148 * 64 ? blocks : 148 * 64);
-    const bool vec = ((uintptr_t)X & 15) == 0 && (ldx * nb::elt_size(x_elt)) % 16 == 0 && ((uintptr_t)codes & 3) == 0 && ldq % 4 == 0;
+    const int64_t groups = rows * (K / 16), blocks = (groups + NT - 1) / NT;
+    if (blocks > 0x7fffffff) return nb_set_error("nemo_mxfp4_quantize: too many values");
+    const bool vec = ((uintptr_t)X & 15) == 0 && (ldx * nb::elt_size(x_elt)) % 16 == 0 && ((uintptr_t)codes & 7) == 0 && ldq % 8 == 0;
+    const bool tiles = K % 128 == 0 && ((uintptr_t)scales & 3) == 0;
     cudaStream_t st = (cudaStream_t)stream;
-    NB_ELT_SWITCH(x_elt, T, nb::launch(vec ? mxfp4_quantize_kernel<T, true> : mxfp4_quantize_kernel<T, false>, grid, NT, 0, st, (const T *)X, ldx, groups,
-                                       (int)(K / 8), codes, ldq, scales));
+    NB_ELT_SWITCH(x_elt, T, {
+        auto kernel = vec ? (tiles ? mxfp4_quantize_kernel<T, true, true> : mxfp4_quantize_kernel<T, true, false>)
+                          : (tiles ? mxfp4_quantize_kernel<T, false, true> : mxfp4_quantize_kernel<T, false, false>);
+        nb::launch(kernel, dim3((unsigned)blocks), NT, 0, st, (const T *)X, ldx, groups, (int)(K / 16), codes, ldq, scales);
+    });
     return nb_check_launch("mxfp4_quantize_kernel");
 }
 
@@ -168,12 +177,11 @@ extern "C" int nemo_mxfp4_dequantize(const uint8_t *codes, int64_t ldq, const ui
                                      void *stream) {
     if (check("nemo_mxfp4_dequantize", Y, y_elt, ldy, rows, K, codes, ldq, scales)) return -1;
     if (rows == 0 || K == 0) return 0;
-    const int64_t groups = rows * (K / 8);
-    const int64_t blocks = (groups + NT - 1) / NT;
-    const int grid = (int)(blocks < 148 * 64 ? blocks : 148 * 64);
-    const bool vec = ((uintptr_t)Y & 15) == 0 && (ldy * nb::elt_size(y_elt)) % 16 == 0 && ((uintptr_t)codes & 3) == 0 && ldq % 4 == 0;
+    const int64_t groups = rows * (K / 16), blocks = (groups + NT - 1) / NT;
+    if (blocks > 0x7fffffff) return nb_set_error("nemo_mxfp4_dequantize: too many values");
+    const bool vec = ((uintptr_t)Y & 15) == 0 && (ldy * nb::elt_size(y_elt)) % 16 == 0 && ((uintptr_t)codes & 7) == 0 && ldq % 8 == 0;
     cudaStream_t st = (cudaStream_t)stream;
-    NB_ELT_SWITCH(y_elt, T, nb::launch(vec ? mxfp4_dequantize_kernel<T, true> : mxfp4_dequantize_kernel<T, false>, grid, NT, 0, st, codes, ldq, scales, groups,
-                                       (int)(K / 8), (T *)Y, ldy));
+    NB_ELT_SWITCH(y_elt, T, nb::launch(vec ? mxfp4_dequantize_kernel<T, true> : mxfp4_dequantize_kernel<T, false>, dim3((unsigned)blocks), NT, 0, st, codes, ldq,
+                                       scales, groups, (int)(K / 16), (T *)Y, ldy));
     return nb_check_launch("mxfp4_dequantize_kernel");
 }

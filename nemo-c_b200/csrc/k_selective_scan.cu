@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
+using namespace nb;
 
 struct ScanArgs {
     const void *x, *dt, *z, *B, *C;
@@ -30,12 +30,6 @@ struct ScanArgs {
     int64_t items;     // single rows: warps; runs: channel tiles of all streams
     int tw, ranks;     // runs: chunks of time in a block, blocks of a cluster
 };
-
-__device__ __forceinline__ float ex2(float v) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
 
 // log(1 + e^v) = max(v, 0) + log1p(e), e = exp(-|v|) <= 1, and log1p(e) = 2 artanh(e / (2 + e)): the
 // argument is at most 1/3, so seven terms of the series leave 1.4e-8 of it. No cancellation at either end.
@@ -179,35 +173,6 @@ int run_step(ScanArgs a, cudaStream_t st) {
 
 // ---- runs of rows ----------------------------------------------------------------------------
 
-typedef unsigned long long f2;  // two fp32 in a register pair
-__device__ __forceinline__ f2 pack2(float lo, float hi) {
-    f2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpack2(f2 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-    f2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-    f2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 dup2(float v) { return pack2(v, v); }
-__device__ __forceinline__ float rcp(float v) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
 // softplus_f of two values
 __device__ __forceinline__ f2 softplus2(f2 v) {
     float a, b;

@@ -24,6 +24,7 @@
 #include <cuda.h>
 #include <cstring>
 #include <cstdlib>
+#include <type_traits>
 #include <atomic>
 #include "cluster.cuh"
 #include "elt.cuh"
@@ -45,7 +46,7 @@ struct MxArgs {
     const float *bias;
     void *C;
     int64_t ldc;
-    int M, N, K, kblocks, katoms, splits, kb_per_split, n_wtiles, n_mtiles, units, act, accumulate;
+    int M, N, K, kblocks, katoms, splits, kb_per_split, n_wtiles, n_mtiles, units, act, accumulate, vec;
     float alpha;
     int *err;
 };
@@ -55,12 +56,15 @@ struct Cfg {
     static constexpr int W_BYTES = BM * BKB, A_BYTES = BN * BKB;
     static constexpr int WS_OFF = WT * W_BYTES + A_BYTES;      // scales: 2 atoms per weight tile, 2 for the activations
     static constexpr int STAGE = WS_OFF + (WT + 1) * 2 * ATOM;
-    static constexpr int STAGES = BN == 128 ? (WT == 2 ? 4 : 6) : (WT == 2 ? 4 : 8);
+    static constexpr int STAGES = WT == 2 ? 4 : BN == 128 ? 6 : BN == 64 ? 7 : 8;
     static constexpr int SLOTS = WT == 1 ? 2 : BN == 128 ? 3 : 4;  // accumulators of BN columns
     static constexpr int SC_COLS = (WT + 1) * 8;                 // scale columns per stage
     static constexpr int COLS = SLOTS * BN + STAGES * SC_COLS;
     static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
+    // 16-bit outputs pass through shared memory: per epilogue warp 32 rows of 32 columns, 80 bytes apart
+    static constexpr int OUT = BN >= 64 ? EPI_WARPS * 32 * 80 : 0;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + OUT + 256;
+    static_assert(SMEM <= 232448, "shared memory");
     static_assert(COLS <= 512, "tensor memory");
     static_assert(STAGE % 1024 == 0, "swizzled tiles start on 1 KB");
     static_assert(WT * BN * BM * 4 <= STAGES * STAGE, "partial tiles reuse the stages");
@@ -72,11 +76,19 @@ __device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t by
                  : "memory");
 }
 
-// Descriptor of a scale tile in shared memory: 32 rows of 16 bytes, contiguous, no swizzle (core
-// matrices of 8 rows x 16 bytes are 128 bytes apart).
-__device__ __forceinline__ uint64_t desc_scale(uint32_t smem_addr) {
-    return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+// Shared-memory descriptors, low word: address / 16 (and a leading offset of 16 bytes, unused, for the
+// operands); the high words are constants, so one thread can issue an MMA every few instructions.
+// Operand tiles: K-major, 128-byte swizzle, groups of 8 rows 1024 bytes apart; 32 bytes of k further on
+// is an address 32 bytes on. Scale tiles: 32 rows of 16 bytes, contiguous, no swizzle (core matrices of
+// 8 rows x 16 bytes are 128 bytes apart).
+constexpr uint32_t OPERAND_HI = (1024 >> 4) | 1u << 14 | 2u << 29, SCALE_HI = (128 >> 4) | 1u << 14;
+__device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
 }
+__device__ __forceinline__ uint64_t desc_operand(uint32_t smem_addr) { return desc64(smem_addr >> 4 | 1u << 16, OPERAND_HI); }
+__device__ __forceinline__ uint64_t desc_scale(uint32_t smem_addr) { return desc64(smem_addr >> 4, SCALE_HI); }
 // 32 lanes x 16 bytes, written to all four 32-lane quarters of tensor memory.
 __device__ __forceinline__ void cp_scale(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
@@ -89,6 +101,7 @@ __host__ __device__ constexpr uint32_t idesc_mxf4(int N, int half) {
            ((uint32_t)(half * 2) << 29);
 }
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+    // (accumulate: constant but for the first MMA of a unit)
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
@@ -124,6 +137,31 @@ __device__ __forceinline__ void tmem_wait_ld(float (&v)[CN]) {
     for (int j = 0; j < CN; ++j) asm volatile("" : "+f"(v[j]));
 }
 
+// 16 lanes x 32 columns in the layout of a matrix fragment: v[4 k + 2 h + e] is lane 8 h + t / 4, column
+// 8 k + 2 (t % 4) + e.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+          "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Four 8 x 8 matrices of 16-bit elements, transposed: thread t names row t % 8 of matrix t / 8.
+__device__ __forceinline__ void store_frag_t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *(const uint32_t *)&h;
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *(const uint32_t *)&h;
+    }
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
 }
@@ -142,30 +180,43 @@ __device__ __forceinline__ void finish(const MxArgs &p, int m, int n, float va, 
     if (p.accumulate) v += nb::to_f32(*c);
     *c = nb::from_f32<T>(v);
 }
-// The same for CN rows of one output column, in pairs; v holds the accumulators, g GLU's gates.
-template <int ACT, int CN>
-__device__ __forceinline__ void activate(float (&v)[CN], const float (&g)[CN], float ba, float bb, float alpha) {
-#pragma unroll
-    for (int j = 0; j < CN; j += 2) {
-        nb::f2 x = nb::add2(nb::pack2(v[j], v[j + 1]), nb::dup2(ba));
-        if (ACT == NEMO_ACT_SILU) x = nb::mul2(x, nb::sigmoid2(x));
-        if (ACT == NEMO_ACT_GLU) x = nb::mul2(x, nb::sigmoid2(nb::add2(nb::pack2(g[j], g[j + 1]), nb::dup2(bb))));
-        if (ACT == NEMO_ACT_RELU) {
-            float a, b;
-            nb::unpack2(x, a, b);
-            x = nb::pack2(a < 0.0f ? 0.0f : a, b < 0.0f ? 0.0f : b);
-        }
-        nb::unpack2(nb::mul2(x, nb::dup2(alpha)), v[j], v[j + 1]);
+// Two rows of one output column; g: GLU's gates.
+template <int ACT>
+__device__ __forceinline__ void activate(float &v0, float &v1, float g0, float g1, float ba, float bb, float alpha) {
+    nb::f2 x = nb::add2(nb::pack2(v0, v1), nb::dup2(ba));
+    if (ACT == NEMO_ACT_SILU) x = nb::mul2(x, nb::sigmoid2(x));
+    if (ACT == NEMO_ACT_GLU) x = nb::mul2(x, nb::sigmoid2(nb::add2(nb::pack2(g0, g1), nb::dup2(bb))));
+    if (ACT == NEMO_ACT_RELU) {
+        float a, b;
+        nb::unpack2(x, a, b);
+        x = nb::pack2(a < 0.0f ? 0.0f : a, b < 0.0f ? 0.0f : b);
     }
+    nb::unpack2(nb::mul2(x, nb::dup2(alpha)), v0, v1);
 }
+// CN rows of one output column.
+template <int ACT, int CN>
+__device__ __forceinline__ void activate_rows(float (&v)[CN], const float (&g)[CN], float ba, float bb, float alpha) {
+#pragma unroll
+    for (int j = 0; j < CN; j += 2) activate<ACT>(v[j], v[j + 1], g[j], g[j + 1], ba, bb, alpha);
+}
+// A fragment (tmem_ld_frag): ba, bb hold the biases of its two lanes.
+template <int ACT>
+__device__ __forceinline__ void activate_frag(float (&v)[16], const float (&g)[16], const float (&ba)[2], const float (&bb)[2], float alpha) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) activate<ACT>(v[2 * k], v[2 * k + 1], g[2 * k], g[2 * k + 1], ba[k & 1], bb[k & 1], alpha);
+}
+#define MX_ACT_SWITCH(act, CALL)                     \
+    switch (act) {                                   \
+        case NEMO_ACT_SILU: CALL(NEMO_ACT_SILU); break; \
+        case NEMO_ACT_RELU: CALL(NEMO_ACT_RELU); break; \
+        case NEMO_ACT_GLU: CALL(NEMO_ACT_GLU); break;   \
+        default: CALL(NEMO_ACT_NONE); break;          \
+    }
 template <typename T, int CN>
 __device__ __forceinline__ void finish_rows(const MxArgs &p, int m, int n, int count, float (&v)[CN], const float (&g)[CN], float ba, float bb) {
-    switch (p.act) {
-        case NEMO_ACT_SILU: activate<NEMO_ACT_SILU, CN>(v, g, ba, bb, p.alpha); break;
-        case NEMO_ACT_RELU: activate<NEMO_ACT_RELU, CN>(v, g, ba, bb, p.alpha); break;
-        case NEMO_ACT_GLU: activate<NEMO_ACT_GLU, CN>(v, g, ba, bb, p.alpha); break;
-        default: activate<NEMO_ACT_NONE, CN>(v, g, ba, bb, p.alpha); break;
-    }
+#define CALL(A) activate_rows<A, CN>(v, g, ba, bb, p.alpha)
+    MX_ACT_SWITCH(p.act, CALL)
+#undef CALL
     T *c = (T *)p.C + (int64_t)m * p.ldc + n;
     if (p.accumulate) {
 #pragma unroll
@@ -188,7 +239,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     using C = Cfg<BN, WT>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *stages = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t *full = (uint64_t *)(stages + C::STAGES * C::STAGE);
+    uint8_t *outs = stages + C::STAGES * C::STAGE;
+    uint64_t *full = (uint64_t *)(outs + C::OUT);
     uint64_t *empty = full + C::STAGES;
     uint64_t *acc_full = empty + C::STAGES;     // [SLOTS] MMA -> epilogue
     uint64_t *acc_empty = acc_full + C::SLOTS;  // [SLOTS] epilogue -> MMA
@@ -267,20 +319,28 @@ __global__ void __launch_bounds__(THREADS, 1)
                 sm100::tc_fence_after();
                 const uint32_t st = sm100::smem_u32(stages + s * C::STAGE);
                 const uint32_t sc = tmem + C::SLOTS * BN + s * C::SC_COLS;
-                const int atoms = min(2, p.katoms - kb * 2), steps = min(4, (p.K - kb * 256 + 63) / 64);
+                auto stage = [&](int atoms, int steps, bool second) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i <= WT; ++i) {  // weight tiles, then the activations
-                    if (i == 1 && WT == 2 && !two) continue;
-                    for (int a = 0; a < atoms; ++a) cp_scale(sc + i * 8 + a * 4, desc_scale(st + C::WS_OFF + (i * 2 + a) * ATOM));
-                }
+                    for (int i = 0; i <= WT; ++i) {  // weight tiles, then the activations
+                        if (i == 1 && WT == 2 && !second) continue;
 #pragma unroll
-                for (int i = 0; i < WT; ++i) {
-                    if (i && !two) break;
-                    const uint32_t d = tmem + ((t * WT + i) % C::SLOTS) * BN;
-                    for (int kk = 0; kk < steps; ++kk)
-                        mma_mxf4(d, sm100::desc_k_sw128(st + i * C::W_BYTES + kk * 32), sm100::desc_k_sw128(st + WT * C::W_BYTES + kk * 32),
-                                 idesc_mxf4(BN, kk & 1), sc + i * 8 + (kk >> 1) * 4, sc + WT * 8 + (kk >> 1) * 4, kb != kb0 || kk != 0);
-                }
+                        for (int a = 0; a < 2; ++a)
+                            if (a < atoms) cp_scale(sc + i * 8 + a * 4, desc_scale(st + C::WS_OFF + (i * 2 + a) * ATOM));
+                    }
+#pragma unroll
+                    for (int i = 0; i < WT; ++i) {
+                        if (i && !second) break;
+                        const uint32_t d = tmem + ((t * WT + i) % C::SLOTS) * BN;
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            if (kk < steps)
+                                mma_mxf4(d, desc_operand(st + i * C::W_BYTES + kk * 32), desc_operand(st + WT * C::W_BYTES + kk * 32), idesc_mxf4(BN, kk & 1),
+                                         sc + i * 8 + (kk >> 1) * 4, sc + WT * 8 + (kk >> 1) * 4, kb != kb0 || kk != 0);
+                    }
+                };
+                const int left = p.K - kb * 256;
+                if (left >= 256 && (WT == 1 || two)) stage(2, 4, WT == 2);
+                else stage(left > 128 ? 2 : 1, min(4, (left + 63) / 64), two);
                 sm100::mma_commit(&empty[s]);
             }
 #pragma unroll
@@ -319,23 +379,70 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                 for (int i = 0; i < WT; ++i) {
                     if (i && glu) break;
-                    const int n = (glu ? wt * BM : wrow(wt, i)) + row;
-                    const bool on = n < nout;
-                    const float ba = on && p.bias ? p.bias[n] : 0.0f, bb = on && glu && p.bias ? p.bias[n + p.N / 2] : 0.0f;
+                    const int n1 = glu ? wt * BM : wrow(wt, i);
                     const uint32_t acc = lanes + ((t * WT + i) % C::SLOTS) * BN, gate = lanes + ((t * WT + 1) % C::SLOTS) * BN;
-                    constexpr int CN = BN >= 64 && WT == 1 ? 32 : 16;  // columns per load
-                    for (int j0 = jbeg; j0 < jend && j0 < mcount; j0 += CN) {
-                        float v[CN], g[CN];
-                        tmem_ld(acc + j0, v);
-                        if (WT == 2 && glu) tmem_ld(gate + j0, g);
-                        tmem_wait_ld(v);
-                        if (WT == 2 && glu) tmem_wait_ld(g);
-                        if (on) finish_rows<T, CN>(p, m0 + j0, n, mcount - j0, v, g, ba, bb);
+                    if (C::OUT && sizeof(T) == 2 && p.vec) {
+                        // fragments of 16 columns x 32 rows, transposed through shared memory into runs of
+                        // eight columns: one 16-byte store where single elements take eight
+                        uint8_t *buf = outs + (warp - 2) * 32 * 80;
+                        const int nq = n1 + q * 32;
+                        float ba[2][2], bb[2][2];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const int n = nq + h * 8 + lane / 4;
+                            ba[h >> 1][h & 1] = n < nout && p.bias ? p.bias[n] : 0.0f;
+                            bb[h >> 1][h & 1] = n < nout && glu && p.bias ? p.bias[n + p.N / 2] : 0.0f;
+                        }
+                        // where this thread's matrix row goes (matrix = lane / 8: columns 8 (m & 1), rows 8 (m / 2))
+                        const uint32_t to = sm100::smem_u32(buf) + (8 * (lane >> 4) + (lane & 7)) * 80 + ((lane >> 3) & 1) * 16;
+                        for (int j0 = jbeg; j0 < jend && j0 < mcount; j0 += 32) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                float v[16], g[16];
+                                tmem_ld_frag(acc + (h << 20) + j0, v);
+                                if (WT == 2 && glu) tmem_ld_frag(gate + (h << 20) + j0, g);
+                                tmem_wait_ld(v);
+                                if (WT == 2 && glu) tmem_wait_ld(g);
+#define CALL(A) activate_frag<A>(v, g, ba[h], bb[h], p.alpha)
+                                MX_ACT_SWITCH(p.act, CALL)
+#undef CALL
+#pragma unroll
+                                for (int k = 0; k < 2; ++k)
+                                    store_frag_t(to + k * 16 * 80 + h * 32, pack16<T>(v[8 * k], v[8 * k + 1]), pack16<T>(v[8 * k + 2], v[8 * k + 3]),
+                                                 pack16<T>(v[8 * k + 4], v[8 * k + 5]), pack16<T>(v[8 * k + 6], v[8 * k + 7]));
+                            }
+                            __syncwarp();
+                            const int n = nq + (lane & 3) * 8;
+                            T *c = (T *)p.C + (int64_t)(m0 + j0 + lane / 4) * p.ldc + n;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint4 o = *(const uint4 *)(buf + (k * 8 + lane / 4) * 80 + (lane & 3) * 16);
+                                if (n < nout && j0 + k * 8 + lane / 4 < mcount) *(uint4 *)(c + k * 8 * p.ldc) = o;
+                            }
+                            __syncwarp();
+                        }
+                    } else {
+                        const int n = n1 + row;
+                        const bool on = n < nout;
+                        const float ba = on && p.bias ? p.bias[n] : 0.0f, bb = on && glu && p.bias ? p.bias[n + p.N / 2] : 0.0f;
+                        constexpr int CN = BN >= 64 && WT == 1 ? 32 : 16;  // columns per load
+                        for (int j0 = jbeg; j0 < jend && j0 < mcount; j0 += CN) {
+                            float v[CN], g[CN];
+                            tmem_ld(acc + j0, v);
+                            if (WT == 2 && glu) tmem_ld(gate + j0, g);
+                            tmem_wait_ld(v);
+                            if (WT == 2 && glu) tmem_wait_ld(g);
+                            if (on) finish_rows<T, CN>(p, m0 + j0, n, mcount - j0, v, g, ba, bb);
+                        }
+                    }
+                    // this accumulator (GLU: both) may be overwritten: the next unit's MMAs need not wait for the other
+                    sm100::tc_fence_before();
+                    sm100::named_barrier(1, 256);
+                    if (etid == 0) {
+                        mbar_arrive(&acc_empty[(t * WT + i) % C::SLOTS]);
+                        if (WT == 2 && glu) mbar_arrive(&acc_empty[(t * WT + 1) % C::SLOTS]);
                     }
                 }
-                sm100::tc_fence_before();
-                sm100::named_barrier(1, 256);
-                if (etid < WT) mbar_arrive(&acc_empty[(t * WT + etid) % C::SLOTS]);
             }
         }
     }
@@ -411,6 +518,7 @@ int run(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
     memset(&p, 0, sizeof p);
     p.as = a->a_scales; p.ws = a->w_scales; p.bias = a->bias; p.C = a->C; p.ldc = a->ldc;
     p.M = a->M; p.N = a->N; p.K = a->K; p.act = a->act; p.accumulate = a->accumulate; p.alpha = a->alpha;
+    p.vec = sizeof(T) == 2 && ((uintptr_t)a->C & 15) == 0 && a->ldc % 8 == 0 && (glu ? a->N / 2 : a->N) % 8 == 0;
     p.kblocks = (a->K + 255) / 256;
     p.katoms = (a->K + 127) / 128;
     const int wspan = glu ? BM : WT * BM;

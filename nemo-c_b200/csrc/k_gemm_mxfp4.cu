@@ -162,6 +162,12 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     }
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
 }
@@ -247,7 +253,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t *tmem_holder = (uint32_t *)(acc_empty + C::SLOTS);
     volatile int *flags = (volatile int *)(tmem_holder + 1);  // [0] a wait gave up, [1] the epilogue's own
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the same in every lane, and known to be: what the issuing warp computes then stays in uniform registers,
+    // which is where the tensor instructions take their operands from
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) { sm100::mbar_init(&full[s], 1); sm100::mbar_init(&empty[s], 1); }
         for (int s = 0; s < C::SLOTS; ++s) { sm100::mbar_init(&acc_full[s], 1); sm100::mbar_init(&acc_empty[s], 1); }
@@ -263,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     sm100::tc_fence_before();
     __syncthreads();
     sm100::tc_fence_after();
-    const uint32_t tmem = *tmem_holder;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_holder, 0);
     nb::pdl_wait();
 
     const bool glu = p.act == NEMO_ACT_GLU;
@@ -273,36 +281,49 @@ __global__ void __launch_bounds__(THREADS, 1)
     // first weight row of tile i of unit u
     auto wrow = [&](int wt, int i) { return glu ? wt * BM + (i ? p.N / 2 : 0) : (wt * WT + i) * BM; };
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
+        const bool leader = elect_one();
         int it = 0;
-        for (int u = u0; u < p.units && !flags[0]; u += ustep) {
+        for (int u = u0; u < p.units; u += ustep) {
             const int mt = u % p.n_mtiles, wt = u / p.n_mtiles;
+            // a second weight tile wholly past the last row is not loaded (its output is not written)
+            const int r0 = wrow(wt, 0), r1 = wrow(wt, 1);
+            const bool two = WT == 2 && r1 < p.N;
+            const uint8_t *ws0 = p.ws + (int64_t)(r0 / BM) * p.katoms * ATOM, *ws1 = p.ws + (int64_t)(r1 / BM) * p.katoms * ATOM;
+            const uint8_t *as = p.as + (int64_t)(mt * BN / 128) * p.katoms * ATOM;
+            bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % C::STAGES;
-                if (it >= C::STAGES && !sm100::mbar_wait(&empty[s], ((it / C::STAGES) - 1) & 1)) { flags[0] = 1; atomicExch(p.err, 5); break; }
-                if (flags[0]) break;
-                uint8_t *st = stages + s * C::STAGE;
-                const uint32_t sb = (uint32_t)min(2, p.katoms - kb * 2) * ATOM;  // scale tiles of these columns
-                // a second weight tile wholly past the last row is not loaded (its output is not written)
-                const bool two = WT == 2 && wrow(wt, 1) < p.N;
-                sm100::mbar_arrive_expect_tx(&full[s], (two ? 2 : 1) * (C::W_BYTES + sb) + C::A_BYTES + sb);
-#pragma unroll
-                for (int i = 0; i < WT; ++i) {
-                    if (i && !two) break;
-                    const int r = wrow(wt, i);
-                    sm100::tma_load_2d(st + i * C::W_BYTES, &tmW, &full[s], kb * BKB, r);
-                    bulk_g2s(st + C::WS_OFF + i * 2 * ATOM, p.ws + ((int64_t)(r / BM) * p.katoms + kb * 2) * ATOM, sb, &full[s]);
+                ok = __all_sync(0xffffffffu, !flags[0] && (it < C::STAGES || sm100::mbar_wait(&empty[s], ((it / C::STAGES) - 1) & 1)));
+                if (!ok) break;
+                if (leader) {
+                    uint8_t *st = stages + s * C::STAGE;
+                    const uint32_t sb = (uint32_t)min(2, p.katoms - kb * 2) * ATOM;  // scale tiles of these columns
+                    sm100::mbar_arrive_expect_tx(&full[s], (two ? 2 : 1) * (C::W_BYTES + sb) + C::A_BYTES + sb);
+                    sm100::tma_load_2d(st, &tmW, &full[s], kb * BKB, r0);
+                    bulk_g2s(st + C::WS_OFF, ws0 + kb * 2 * ATOM, sb, &full[s]);
+                    if (two) {
+                        sm100::tma_load_2d(st + C::W_BYTES, &tmW, &full[s], kb * BKB, r1);
+                        bulk_g2s(st + C::WS_OFF + 2 * ATOM, ws1 + kb * 2 * ATOM, sb, &full[s]);
+                    }
+                    sm100::tma_load_2d(st + WT * C::W_BYTES, &tmA, &full[s], kb * BKB, mt * BN);
+                    bulk_g2s(st + C::WS_OFF + WT * 2 * ATOM, as + kb * 2 * ATOM, sb, &full[s]);
                 }
-                sm100::tma_load_2d(st + WT * C::W_BYTES, &tmA, &full[s], kb * BKB, mt * BN);
-                bulk_g2s(st + C::WS_OFF + WT * 2 * ATOM, p.as + ((int64_t)(mt * BN / 128) * p.katoms + kb * 2) * ATOM, sb, &full[s]);
+                __syncwarp();
+            }
+            if (!ok) {
+                if (!flags[0]) { flags[0] = 1; atomicExch(p.err, 5); }
+                break;
             }
         }
         // a launch that gave up waits for its own copies before its shared memory goes away
-        if (flags[0])
+        if (__any_sync(0xffffffffu, flags[0]))
             for (int j = max(0, it - C::STAGES); j < it; ++j) sm100::mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, 100000000LL);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
+        const bool leader = elect_one();
         int it = 0, t = 0;
-        for (int u = u0; u < p.units && !flags[0]; u += ustep, ++t) {
+        for (int u = u0; u < p.units; u += ustep, ++t) {
+            if (__any_sync(0xffffffffu, flags[0])) break;
             const int wt = u / p.n_mtiles;
             const bool two = WT == 2 && wrow(wt, 1) < p.N;
             bool ok = true;
@@ -311,11 +332,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int q = t * WT + i;
                 if (q >= C::SLOTS && !sm100::mbar_wait(&acc_empty[q % C::SLOTS], ((q / C::SLOTS) - 1) & 1)) ok = false;
             }
-            if (!ok) { flags[0] = 1; atomicExch(p.err, 6); break; }
+            if (!__all_sync(0xffffffffu, ok)) { flags[0] = 1; atomicExch(p.err, 6); break; }
             sm100::tc_fence_after();
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % C::STAGES;
-                if (!sm100::mbar_wait(&full[s], (it / C::STAGES) & 1)) { flags[0] = 1; atomicExch(p.err, 7); break; }
+                if (!__all_sync(0xffffffffu, sm100::mbar_wait(&full[s], (it / C::STAGES) & 1))) { flags[0] = 1; atomicExch(p.err, 7); break; }
                 sm100::tc_fence_after();
                 const uint32_t st = sm100::smem_u32(stages + s * C::STAGE);
                 const uint32_t sc = tmem + C::SLOTS * BN + s * C::SC_COLS;
@@ -339,12 +360,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                 };
                 const int left = p.K - kb * 256;
-                if (left >= 256 && (WT == 1 || two)) stage(2, 4, WT == 2);
-                else stage(left > 128 ? 2 : 1, min(4, (left + 63) / 64), two);
-                sm100::mma_commit(&empty[s]);
+                if (leader) {
+                    if (left >= 256 && (WT == 1 || two)) stage(2, 4, WT == 2);
+                    else stage(left > 128 ? 2 : 1, min(4, (left + 63) / 64), two);
+                    sm100::mma_commit(&empty[s]);
+                }
+                __syncwarp();
             }
+            if (leader)
 #pragma unroll
-            for (int i = 0; i < WT; ++i) sm100::mma_commit(&acc_full[(t * WT + i) % C::SLOTS]);
+                for (int i = 0; i < WT; ++i) sm100::mma_commit(&acc_full[(t * WT + i) % C::SLOTS]);
+            __syncwarp();
         }
     } else if (warp >= 2) {
         const int q = warp & 3, half = (warp - 2) >> 2;  // the 32 lanes and the half of the columns of this warp

@@ -22,4 +22,12 @@ __device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
     return v;
 }
 
+__device__ __forceinline__ float4 ld_cluster4(uint32_t local, uint32_t rank) {
+    uint32_t a;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+
 }  // namespace nb

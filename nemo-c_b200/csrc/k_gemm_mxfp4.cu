@@ -7,13 +7,12 @@
 // columns, so that one kernel serves one row and thousands: a warp's 32 lanes hold 32 neighbouring
 // output columns of an output row, and each store of the epilogue is one contiguous run.
 //
-// A unit of work is WT weight tiles of 128 rows (two for GLU: value rows n and gate rows n + N/2;
-// two also for many activation rows, which then cross L2 -> SM once for 256 weight rows) by one
-// tile of BN activation rows. One stage holds 256 columns of k: the weight and activation codes,
-// brought in by TMA with the 128-byte swizzle, and their scale tiles, one bulk copy each. The MMA
-// thread copies the scales from shared to tensor memory (tcgen05.cp; each stage has tensor-memory
-// columns of its own, so a later stage's copy never meets an MMA that still reads them) and issues
-// four MMAs of 64 columns per weight tile.
+// A unit of work is one weight tile of 128 rows (GLU: two, value rows n and gate rows n + N/2) by one
+// tile of BN activation rows. One stage holds 256 columns of k: the weight and activation codes, brought
+// in by TMA with the 128-byte swizzle, and their scale tiles, one bulk copy each. The MMA thread copies the
+// scales from shared to tensor memory (tcgen05.cp; each stage has tensor-memory columns of its own,
+// so a later stage's copy never meets an MMA that still reads them) and issues four MMAs of 64 columns per
+// weight tile.
 //
 // Few units: a cluster of 2, 4 or 8 CTAs splits k; the partial tiles meet in shared memory across
 // the cluster and are added in the order of their ranks, so results do not depend on scheduling.
@@ -23,7 +22,6 @@
 // error, takes part in the remaining cluster barriers and unwinds.
 #include <cuda.h>
 #include <cstring>
-#include <cstdlib>
 #include <type_traits>
 #include <atomic>
 #include "cluster.cuh"
@@ -110,22 +108,12 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uin
         : "memory");
 }
 
-// 32 lanes x CN consecutive columns; the values are there after tmem_wait_ld.
+// 32 lanes x 16 consecutive columns; the values are there after tmem_wait_ld.
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
           "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
-        "%28,%29,%30,%31}, [%32];"
-        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
-          "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]),
-          "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
         : "r"(taddr)
         : "memory");
 }
@@ -207,7 +195,7 @@ __device__ __forceinline__ void activate_rows(float (&v)[CN], const float (&g)[C
 }
 // A fragment (tmem_ld_frag): ba, bb hold the biases of its two lanes.
 template <int ACT>
-__device__ __forceinline__ void activate_frag(float (&v)[16], const float (&g)[16], const float (&ba)[2], const float (&bb)[2], float alpha) {
+__device__ __forceinline__ void activate_frag(float (&v)[16], const float (&g)[16], const float *ba, const float *bb, float alpha) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) activate<ACT>(v[2 * k], v[2 * k + 1], g[2 * k], g[2 * k + 1], ba[k & 1], bb[k & 1], alpha);
 }
@@ -274,21 +262,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_holder, 0);
     nb::pdl_wait();
 
-    const bool glu = p.act == NEMO_ACT_GLU;
+    constexpr bool glu = WT == 2;
     const int rank = p.splits > 1 ? (int)nb::cluster_rank() : 0;
     const int u0 = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x, ustep = p.splits > 1 ? p.units : gridDim.x;
     const int kb0 = rank * p.kb_per_split, kb1 = min(p.kblocks, kb0 + p.kb_per_split);
     // first weight row of tile i of unit u
-    auto wrow = [&](int wt, int i) { return glu ? wt * BM + (i ? p.N / 2 : 0) : (wt * WT + i) * BM; };
+    auto wrow = [&](int wt, int i) { return wt * BM + (i ? p.N / 2 : 0); };
 
     if (warp == 0) {
         const bool leader = elect_one();
         int it = 0;
         for (int u = u0; u < p.units; u += ustep) {
             const int mt = u % p.n_mtiles, wt = u / p.n_mtiles;
-            // a second weight tile wholly past the last row is not loaded (its output is not written)
             const int r0 = wrow(wt, 0), r1 = wrow(wt, 1);
-            const bool two = WT == 2 && r1 < p.N;
             const uint8_t *ws0 = p.ws + (int64_t)(r0 / BM) * p.katoms * ATOM, *ws1 = p.ws + (int64_t)(r1 / BM) * p.katoms * ATOM;
             const uint8_t *as = p.as + (int64_t)(mt * BN / 128) * p.katoms * ATOM;
             bool ok = true;
@@ -299,10 +285,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (leader) {
                     uint8_t *st = stages + s * C::STAGE;
                     const uint32_t sb = (uint32_t)min(2, p.katoms - kb * 2) * ATOM;  // scale tiles of these columns
-                    sm100::mbar_arrive_expect_tx(&full[s], (two ? 2 : 1) * (C::W_BYTES + sb) + C::A_BYTES + sb);
+                    sm100::mbar_arrive_expect_tx(&full[s], WT * (C::W_BYTES + sb) + C::A_BYTES + sb);
                     sm100::tma_load_2d(st, &tmW, &full[s], kb * BKB, r0);
                     bulk_g2s(st + C::WS_OFF, ws0 + kb * 2 * ATOM, sb, &full[s]);
-                    if (two) {
+                    if (glu) {
                         sm100::tma_load_2d(st + C::W_BYTES, &tmW, &full[s], kb * BKB, r1);
                         bulk_g2s(st + C::WS_OFF + 2 * ATOM, ws1 + kb * 2 * ATOM, sb, &full[s]);
                     }
@@ -324,8 +310,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         int it = 0, t = 0;
         for (int u = u0; u < p.units; u += ustep, ++t) {
             if (__any_sync(0xffffffffu, flags[0])) break;
-            const int wt = u / p.n_mtiles;
-            const bool two = WT == 2 && wrow(wt, 1) < p.N;
             bool ok = true;
 #pragma unroll
             for (int i = 0; i < WT; ++i) {
@@ -340,17 +324,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                 sm100::tc_fence_after();
                 const uint32_t st = sm100::smem_u32(stages + s * C::STAGE);
                 const uint32_t sc = tmem + C::SLOTS * BN + s * C::SC_COLS;
-                auto stage = [&](int atoms, int steps, bool second) __attribute__((always_inline)) {
+                auto stage = [&](int atoms, int steps) __attribute__((always_inline)) {
 #pragma unroll
                     for (int i = 0; i <= WT; ++i) {  // weight tiles, then the activations
-                        if (i == 1 && WT == 2 && !second) continue;
 #pragma unroll
                         for (int a = 0; a < 2; ++a)
                             if (a < atoms) cp_scale(sc + i * 8 + a * 4, desc_scale(st + C::WS_OFF + (i * 2 + a) * ATOM));
                     }
 #pragma unroll
                     for (int i = 0; i < WT; ++i) {
-                        if (i && !second) break;
                         const uint32_t d = tmem + ((t * WT + i) % C::SLOTS) * BN;
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
@@ -361,8 +343,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 };
                 const int left = p.K - kb * 256;
                 if (leader) {
-                    if (left >= 256 && (WT == 1 || two)) stage(2, 4, WT == 2);
-                    else stage(left > 128 ? 2 : 1, min(4, (left + 63) / 64), two);
+                    if (left >= 256) stage(2, 4);
+                    else stage(left > 128 ? 2 : 1, min(4, (left + 63) / 64));
                     sm100::mma_commit(&empty[s]);
                 }
                 __syncwarp();
@@ -381,6 +363,19 @@ __global__ void __launch_bounds__(THREADS, 1)
         int t = 0;
         for (int u = u0; u < p.units; u += ustep, ++t) {
             const int mt = u % p.n_mtiles, wt = u / p.n_mtiles, m0 = mt * BN, mcount = min(BN, p.M - m0);
+            // biases first: they arrive while the unit's products are formed. One per lane, or (FRAG) those of
+            // the fragments' lanes 8 h + lane / 4.
+            const bool frag = C::OUT && sizeof(T) == 2 && p.vec;
+            float ba[WT][4], bb[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+#pragma unroll
+                for (int i = 0; i < WT; ++i) {
+                    const int n = wrow(wt, i) + q * 32 + (frag ? h * 8 + lane / 4 : lane);
+                    ba[i][h] = p.bias && n < p.N && (frag || h == 0) ? p.bias[n] : 0.0f;
+                }
+                bb[h] = glu ? ba[WT - 1][h] : 0.0f;  // of the gates
+            }
             bool good = true;
 #pragma unroll
             for (int i = 0; i < WT; ++i)
@@ -402,72 +397,69 @@ __global__ void __launch_bounds__(THREADS, 1)
                         for (int jj = 0; jj < 16; ++jj) part[(i * BN + j0 + jj) * BM + row] = v[jj];
                     }
             } else {
+                // The warp's whole share to registers at once; then the accumulator (GLU: and its gates') is free for the
+                // MMAs of a later unit, before anything is computed or stored.
+                constexpr int CH = HALF / 16;
+                float v[CH][16], g[CH][16];
+                const uint32_t acc = lanes + (t * WT % C::SLOTS) * BN + jbeg, gate = lanes + ((t * WT + 1) % C::SLOTS) * BN + jbeg;
+                const bool mine = jbeg < BN;
+                if (mine) {
 #pragma unroll
-                for (int i = 0; i < WT; ++i) {
-                    if (i && glu) break;
-                    const int n1 = glu ? wt * BM : wrow(wt, i);
-                    const uint32_t acc = lanes + ((t * WT + i) % C::SLOTS) * BN, gate = lanes + ((t * WT + 1) % C::SLOTS) * BN;
-                    if (C::OUT && sizeof(T) == 2 && p.vec) {
-                        // fragments of 16 columns x 32 rows, transposed through shared memory into runs of
-                        // eight columns: one 16-byte store where single elements take eight
-                        uint8_t *buf = outs + (warp - 2) * 32 * 80;
-                        const int nq = n1 + q * 32;
-                        float ba[2][2], bb[2][2];
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            const int n = nq + h * 8 + lane / 4;
-                            ba[h >> 1][h & 1] = n < nout && p.bias ? p.bias[n] : 0.0f;
-                            bb[h >> 1][h & 1] = n < nout && glu && p.bias ? p.bias[n + p.N / 2] : 0.0f;
+                    for (int k = 0; k < CH; ++k) {
+                        // fragments: columns 32 (k / 2), lanes 16 (k & 1); rows: columns 16 k
+                        if (frag) tmem_ld_frag(acc + (k >> 1) * 32 + ((k & 1) << 20), v[k]);
+                        else tmem_ld(acc + k * 16, v[k]);
+                        if (glu) {
+                            if (frag) tmem_ld_frag(gate + (k >> 1) * 32 + ((k & 1) << 20), g[k]);
+                            else tmem_ld(gate + k * 16, g[k]);
                         }
-                        // where this thread's matrix row goes (matrix = lane / 8: columns 8 (m & 1), rows 8 (m / 2))
-                        const uint32_t to = sm100::smem_u32(buf) + (8 * (lane >> 4) + (lane & 7)) * 80 + ((lane >> 3) & 1) * 16;
-                        for (int j0 = jbeg; j0 < jend && j0 < mcount; j0 += 32) {
+                    }
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                float v[16], g[16];
-                                tmem_ld_frag(acc + (h << 20) + j0, v);
-                                if (WT == 2 && glu) tmem_ld_frag(gate + (h << 20) + j0, g);
-                                tmem_wait_ld(v);
-                                if (WT == 2 && glu) tmem_wait_ld(g);
-#define CALL(A) activate_frag<A>(v, g, ba[h], bb[h], p.alpha)
-                                MX_ACT_SWITCH(p.act, CALL)
+                    for (int k = 0; k < CH; ++k) {
+                        tmem_wait_ld(v[k]);
+                        if (glu) tmem_wait_ld(g[k]);
+                    }
+                }
+                sm100::tc_fence_before();
+                sm100::named_barrier(1, 256);
+                if (etid < WT) mbar_arrive(&acc_empty[(t * WT + etid) % C::SLOTS]);
+                if (!mine) continue;
+                const int n1 = wt * BM;
+                if (frag) {
+                    // transposed through shared memory into runs of eight columns: one 16-byte store where
+                    // single elements take eight
+                    uint8_t *buf = outs + (warp - 2) * 32 * 80;
+                    const int nq = n1 + q * 32;
+                    // where this thread's matrix row goes (matrix = lane / 8: columns 8 (m & 1), rows 8 (m / 2))
+                    const uint32_t to = sm100::smem_u32(buf) + (8 * (lane >> 4) + (lane & 7)) * 80 + ((lane >> 3) & 1) * 16;
+#pragma unroll
+                    for (int c0 = 0; c0 < CH; c0 += 2) {
+                        if (jbeg + c0 * 16 >= mcount) break;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float(&vv)[16] = v[c0 + h];
+#define CALL(A) activate_frag<A>(vv, g[c0 + h], &ba[0][2 * h], &bb[2 * h], p.alpha)
+                            MX_ACT_SWITCH(p.act, CALL)
 #undef CALL
 #pragma unroll
-                                for (int k = 0; k < 2; ++k)
-                                    store_frag_t(to + k * 16 * 80 + h * 32, pack16<T>(v[8 * k], v[8 * k + 1]), pack16<T>(v[8 * k + 2], v[8 * k + 3]),
-                                                 pack16<T>(v[8 * k + 4], v[8 * k + 5]), pack16<T>(v[8 * k + 6], v[8 * k + 7]));
-                            }
-                            __syncwarp();
-                            const int n = nq + (lane & 3) * 8;
-                            T *c = (T *)p.C + (int64_t)(m0 + j0 + lane / 4) * p.ldc + n;
+                            for (int k = 0; k < 2; ++k)
+                                store_frag_t(to + k * 16 * 80 + h * 32, pack16<T>(vv[8 * k], vv[8 * k + 1]), pack16<T>(vv[8 * k + 2], vv[8 * k + 3]),
+                                             pack16<T>(vv[8 * k + 4], vv[8 * k + 5]), pack16<T>(vv[8 * k + 6], vv[8 * k + 7]));
+                        }
+                        __syncwarp();
+                        const int n = nq + (lane & 3) * 8, j0 = jbeg + c0 * 16;
+                        T *c = (T *)p.C + (int64_t)(m0 + j0 + lane / 4) * p.ldc + n;
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint4 o = *(const uint4 *)(buf + (k * 8 + lane / 4) * 80 + (lane & 3) * 16);
-                                if (n < nout && j0 + k * 8 + lane / 4 < mcount) *(uint4 *)(c + k * 8 * p.ldc) = o;
-                            }
-                            __syncwarp();
+                        for (int k = 0; k < 4; ++k) {
+                            const uint4 o = *(const uint4 *)(buf + (k * 8 + lane / 4) * 80 + (lane & 3) * 16);
+                            if (n < nout && j0 + k * 8 + lane / 4 < mcount) *(uint4 *)(c + k * 8 * p.ldc) = o;
                         }
-                    } else {
-                        const int n = n1 + row;
-                        const bool on = n < nout;
-                        const float ba = on && p.bias ? p.bias[n] : 0.0f, bb = on && glu && p.bias ? p.bias[n + p.N / 2] : 0.0f;
-                        constexpr int CN = BN >= 64 && WT == 1 ? 32 : 16;  // columns per load
-                        for (int j0 = jbeg; j0 < jend && j0 < mcount; j0 += CN) {
-                            float v[CN], g[CN];
-                            tmem_ld(acc + j0, v);
-                            if (WT == 2 && glu) tmem_ld(gate + j0, g);
-                            tmem_wait_ld(v);
-                            if (WT == 2 && glu) tmem_wait_ld(g);
-                            if (on) finish_rows<T, CN>(p, m0 + j0, n, mcount - j0, v, g, ba, bb);
-                        }
+                        __syncwarp();
                     }
-                    // this accumulator (GLU: both) may be overwritten: the next unit's MMAs need not wait for the other
-                    sm100::tc_fence_before();
-                    sm100::named_barrier(1, 256);
-                    if (etid == 0) {
-                        mbar_arrive(&acc_empty[(t * WT + i) % C::SLOTS]);
-                        if (WT == 2 && glu) mbar_arrive(&acc_empty[(t * WT + 1) % C::SLOTS]);
-                    }
+                } else if (n1 + row < nout) {
+#pragma unroll
+                    for (int k = 0; k < CH; ++k)
+                        if (jbeg + k * 16 < mcount) finish_rows<T, 16>(p, m0 + jbeg + k * 16, n1 + row, mcount - jbeg - k * 16, v[k], g[k], ba[0][0], bb[0]);
                 }
             }
         }
@@ -478,19 +470,33 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncthreads();
         nb::cluster_sync();
         const int mt = u0 % p.n_mtiles, wt = u0 / p.n_mtiles, m0 = mt * BN, mcount = min(BN, p.M - m0);
-        const int nout = glu ? p.N / 2 : p.N, total = (glu || WT == 1 ? 1 : WT) * mcount * BM;
-        const uint32_t part = sm100::smem_u32(stages);
-        if (!flags[0])
-            for (int e = rank * THREADS + threadIdx.x; e < total; e += p.splits * THREADS) {
-                const int row = e % BM, j = e / BM % mcount, i = e / BM / mcount;
-                const int n = (glu ? wt * BM : wrow(wt, i)) + row;
-                if (n >= nout) continue;
-                float v = 0.0f, g = 0.0f;
-                for (int r = 0; r < p.splits; ++r) {
-                    v += nb::ld_cluster(part + ((i * BN + j) * BM + row) * 4, r);
-                    if (WT == 2 && glu) g += nb::ld_cluster(part + ((BN + j) * BM + row) * 4, r);
-                }
-                finish<T>(p, m0 + j, n, v, g, p.bias ? p.bias[n] : 0.0f, glu && p.bias ? p.bias[n + p.N / 2] : 0.0f);
+        // a warp takes a column at a time, four neighbouring lanes of the tile per thread, the ranks' partials in order
+        const int nout = glu ? p.N / 2 : p.N, per = (mcount + p.splits - 1) / p.splits;
+        const int j1 = min(mcount, (rank + 1) * per), n = wt * BM + lane * 4;
+        float base[4], bgate[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            base[k] = p.bias && n + k < nout ? p.bias[n + k] : 0.0f;
+            bgate[k] = glu && p.bias && n + k < nout ? p.bias[n + k + p.N / 2] : 0.0f;
+        }
+        const uint32_t part = sm100::smem_u32(stages) + lane * 16;
+        if (!flags[0] && n < nout)
+            for (int j = rank * per + warp; j < j1; j += THREADS / 32) {
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f), g = v;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < p.splits) {
+                        const float4 a = nb::ld_cluster4(part + j * BM * 4, r);
+                        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+                        if (glu) {
+                            const float4 b = nb::ld_cluster4(part + (BN + j) * BM * 4, r);
+                            g.x += b.x; g.y += b.y; g.z += b.z; g.w += b.w;
+                        }
+                    }
+                const float vv[4] = { v.x, v.y, v.z, v.w }, gg[4] = { g.x, g.y, g.z, g.w };
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (n + k < nout) finish<T>(p, m0 + j, n + k, vv[k], gg[k], base[k], bgate[k]);
             }
         nb::cluster_sync();  // no CTA leaves while another reads its shared memory
     }
@@ -534,7 +540,7 @@ int code_map(CUtensorMap *m, const uint8_t *base, int64_t K, int64_t rows, int64
 template <typename T, int BN, int WT>
 int run(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
     using C = Cfg<BN, WT>;
-    const bool glu = a->act == NEMO_ACT_GLU;
+    constexpr bool glu = WT == 2;
     CUtensorMap mw, ma;
     if (code_map(&mw, a->W, a->K, a->N, a->ldw, BM) || code_map(&ma, a->A, a->K, a->M, a->lda, BN)) return -1;
     int dev = 0, sms = 0;
@@ -547,8 +553,7 @@ int run(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
     p.vec = sizeof(T) == 2 && ((uintptr_t)a->C & 15) == 0 && a->ldc % 8 == 0 && (glu ? a->N / 2 : a->N) % 8 == 0;
     p.kblocks = (a->K + 255) / 256;
     p.katoms = (a->K + 127) / 128;
-    const int wspan = glu ? BM : WT * BM;
-    p.n_wtiles = ((glu ? a->N / 2 : a->N) + wspan - 1) / wspan;
+    p.n_wtiles = ((glu ? a->N / 2 : a->N) + BM - 1) / BM;
     p.n_mtiles = (a->M + BN - 1) / BN;
     const int64_t units = (int64_t)p.n_wtiles * p.n_mtiles;
     if (units > 0x3fffffff) return nb_set_error("nemo_gemm_mxfp4: too many tiles");
@@ -592,15 +597,6 @@ int run(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
 template <typename T>
 int by_rows(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
     const bool glu = a->act == NEMO_ACT_GLU;
-    const char *e = getenv("MXCFG");
-    if (e) {
-        int bn = atoi(e), wt = atoi(strchr(e, ',') + 1);
-        if (glu) wt = 2;
-        if (bn == 16 && a->M <= 16) return wt == 1 ? run<T, 16, 1>(a, st) : run<T, 16, 2>(a, st);
-        if (bn == 32 && a->M <= 32) return wt == 1 ? run<T, 32, 1>(a, st) : run<T, 32, 2>(a, st);
-        if (bn == 64 && a->M <= 64) return wt == 1 ? run<T, 64, 1>(a, st) : run<T, 64, 2>(a, st);
-        if (bn == 128) return wt == 1 ? run<T, 128, 1>(a, st) : run<T, 128, 2>(a, st);
-    }
     if (a->M <= 16) return glu ? run<T, 16, 2>(a, st) : run<T, 16, 1>(a, st);
     if (a->M <= 64) return glu ? run<T, 64, 2>(a, st) : run<T, 64, 1>(a, st);
     return glu ? run<T, 128, 2>(a, st) : run<T, 128, 1>(a, st);

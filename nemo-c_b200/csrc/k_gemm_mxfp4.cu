@@ -17,8 +17,8 @@
 // Few units: a cluster of 2, 4 or 8 CTAs splits k; the partial tiles meet in shared memory across
 // the cluster and are added in the order of their ranks, so results do not depend on scheduling.
 // Otherwise persistent CTAs walk the units, the epilogue of one running beside the MMAs of the
-// next. Warp roles (320 threads): warp 0 loads, warp 1 owns tensor memory and issues the MMAs,
-// warps 2-9 run the epilogue. Every wait on a barrier is bounded: on a timeout the CTA records an
+// next. Warp roles: warp 0 loads, warp 1 owns tensor memory and issues the MMAs, the others run
+// the epilogue. Every wait on a barrier is bounded: on a timeout the CTA records an
 // error, takes part in the remaining cluster barriers and unwinds.
 #include <cuda.h>
 #include <cstring>
@@ -35,8 +35,6 @@ namespace {
 
 constexpr int BM = 128;   // weight rows per tile
 constexpr int BKB = 128;  // code bytes per row and stage: 256 columns of k, one swizzle span
-constexpr int EPI_WARPS = 8;
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int ATOM = 512; // bytes of one scale tile (128 rows x 128 columns of k)
 
 struct MxArgs {
@@ -51,16 +49,19 @@ struct MxArgs {
 
 template <int BN, int WT>
 struct Cfg {
+    // Epilogue groups of 8 warps, which take units in turn: two where units are large and many, so that one
+    // group's activations run beside the other's loads and stores (the registers of GLU allow one)
+    static constexpr int GROUPS = BN == 128 && WT == 1 ? 2 : 1, THREADS = 64 + 256 * GROUPS;
     static constexpr int W_BYTES = BM * BKB, A_BYTES = BN * BKB;
     static constexpr int WS_OFF = WT * W_BYTES + A_BYTES;      // scales: 2 atoms per weight tile, 2 for the activations
     static constexpr int STAGE = WS_OFF + (WT + 1) * 2 * ATOM;
-    static constexpr int STAGES = WT == 2 ? 4 : BN == 128 ? 6 : BN == 64 ? 7 : 8;
+    static constexpr int STAGES = WT == 2 ? 4 : BN == 128 ? 5 : BN == 64 ? 7 : 8;
     static constexpr int SLOTS = WT == 1 ? 2 : BN == 128 ? 3 : 4;  // accumulators of BN columns
     static constexpr int SC_COLS = (WT + 1) * 8;                 // scale columns per stage
     static constexpr int COLS = SLOTS * BN + STAGES * SC_COLS;
     static constexpr int TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     // 16-bit outputs pass through shared memory: per epilogue warp 32 rows of 32 columns, 80 bytes apart
-    static constexpr int OUT = BN >= 64 ? EPI_WARPS * 32 * 80 : 0;
+    static constexpr int OUT = BN >= 64 ? GROUPS * 8 * 32 * 80 : 0;
     static constexpr int SMEM = 1024 + STAGES * STAGE + OUT + 256;
     static_assert(SMEM <= 232448, "shared memory");
     static_assert(COLS <= 512, "tensor memory");
@@ -228,7 +229,7 @@ __device__ __forceinline__ void finish_rows(const MxArgs &p, int m, int n, int c
 }
 
 template <typename T, int BN, int WT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
     gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const __grid_constant__ MxArgs p) {
     using C = Cfg<BN, WT>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t *acc_full = empty + C::STAGES;     // [SLOTS] MMA -> epilogue
     uint64_t *acc_empty = acc_full + C::SLOTS;  // [SLOTS] epilogue -> MMA
     uint32_t *tmem_holder = (uint32_t *)(acc_empty + C::SLOTS);
-    volatile int *flags = (volatile int *)(tmem_holder + 1);  // [0] a wait gave up, [1] the epilogue's own
+    volatile int *flags = (volatile int *)(tmem_holder + 1);  // [0] a wait gave up, [1 + group] an epilogue group's own
 
     // the same in every lane, and known to be: what the issuing warp computes then stays in uniform registers,
     // which is where the tensor instructions take their operands from
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) { sm100::mbar_init(&full[s], 1); sm100::mbar_init(&empty[s], 1); }
         for (int s = 0; s < C::SLOTS; ++s) { sm100::mbar_init(&acc_full[s], 1); sm100::mbar_init(&acc_empty[s], 1); }
-        flags[0] = flags[1] = 0;
+        flags[0] = flags[1] = flags[2] = 0;
         sm100::fence_mbar_init();
         sm100::tma_prefetch_desc(&tmW);
         sm100::tma_prefetch_desc(&tmA);
@@ -355,13 +356,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             __syncwarp();
         }
     } else if (warp >= 2) {
-        const int q = warp & 3, half = (warp - 2) >> 2;  // the 32 lanes and the half of the columns of this warp
-        const int row = q * 32 + lane, etid = threadIdx.x - 64;
+        const int group = (warp - 2) >> 3, q = warp & 3, half = ((warp - 2) >> 2) & 1;  // the 32 lanes and the half of the columns of this warp
+        const int row = q * 32 + lane, etid = (threadIdx.x - 64) & 255;
         constexpr int HALF = BN >= 32 ? BN / 2 : BN;
-        const int jbeg = half * HALF, jend = half * HALF < BN ? jbeg + HALF : jbeg;
+        const int jbeg = half * HALF, jend = jbeg < BN ? jbeg + HALF : jbeg;
         const int nout = glu ? p.N / 2 : p.N;
-        int t = 0;
-        for (int u = u0; u < p.units; u += ustep, ++t) {
+        int t = group;
+        for (int u = u0 + group * ustep; u < p.units; u += C::GROUPS * ustep, t += C::GROUPS) {
             const int mt = u % p.n_mtiles, wt = u / p.n_mtiles, m0 = mt * BN, mcount = min(BN, p.M - m0);
             // biases first: they arrive while the unit's products are formed. One per lane, or (FRAG) those of
             // the fragments' lanes 8 h + lane / 4.
@@ -380,10 +381,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int i = 0; i < WT; ++i)
                 if (!sm100::mbar_wait(&acc_full[(t * WT + i) % C::SLOTS], ((t * WT + i) / C::SLOTS) & 1)) good = false;
-            if (!good) { flags[1] = 1; flags[0] = 1; atomicExch(p.err, 8); }
-            // flags[1] is written only by epilogue threads before this barrier: all of them decide alike
-            sm100::named_barrier(1, 256);
-            if (flags[1]) break;
+            if (!good) { flags[1 + group] = 1; flags[0] = 1; atomicExch(p.err, 8); }
+            // the group's flag is written only by its threads before this barrier: all of them decide alike
+            sm100::named_barrier(1 + group, 256);
+            if (flags[1 + group]) break;
             sm100::tc_fence_after();
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
             if (p.splits > 1) {  // partial tiles to shared memory: [tile][column][lane]
@@ -421,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                 }
                 sm100::tc_fence_before();
-                sm100::named_barrier(1, 256);
+                sm100::named_barrier(1 + group, 256);
                 if (etid < WT) mbar_arrive(&acc_empty[(t * WT + etid) % C::SLOTS]);
                 if (!mine) continue;
                 const int n1 = wt * BM;
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         const uint32_t part = sm100::smem_u32(stages) + lane * 16;
         if (!flags[0] && n < nout)
-            for (int j = rank * per + warp; j < j1; j += THREADS / 32) {
+            for (int j = rank * per + warp; j < j1; j += C::THREADS / 32) {
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f), g = v;
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
@@ -558,14 +559,21 @@ int run(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
     const int64_t units = (int64_t)p.n_wtiles * p.n_mtiles;
     if (units > 0x3fffffff) return nb_set_error("nemo_gemm_mxfp4: too many tiles");
     p.units = (int)units;
-    // k is split while the CTAs of all units still fit the SMs at once and each keeps a stage
+    // k is split over a cluster while the CTAs fit the SMs and the k-blocks saved (0.16 us each) pay for
+    // joining the partial tiles (about 1 us + 7 ns per column and rank): M = 1, N = 1024, K = 4096 takes 5.9 us
+    // whole and 4.9 us in 8 parts, but M = 7, N = 2048, K = 1024 4.0 and 5.3 us, and M = 256, N = 1024, K = 4096 7.5
+    // and 14.2 us.
     int splits = 1;
-    while (splits < 8 && p.units * splits * 2 <= sms && splits * 2 <= p.kblocks) splits *= 2;
-    p.kb_per_split = (p.kblocks + splits - 1) / splits;
-    while (splits > 1 && (splits - 1) * p.kb_per_split >= p.kblocks) {  // every rank has k-blocks
-        splits /= 2;
-        p.kb_per_split = (p.kblocks + splits - 1) / splits;
+    float best = 0.16f * p.kblocks;
+    for (int s = 2; s <= 8 && p.units * s <= sms && s <= p.kblocks; s *= 2) {
+        const int per = (p.kblocks + s - 1) / s;
+        const float cost = 0.16f * per + 1.0f + 0.007f * BN * s;
+        if (cost < best && (s - 1) * per < p.kblocks) {  // every rank has k-blocks
+            best = cost;
+            splits = s;
+        }
     }
+    p.kb_per_split = (p.kblocks + splits - 1) / splits;
     p.splits = splits;
     p.err = nb_tc_error_ptr();
     if (!p.err) return nb_set_error("nemo_gemm_mxfp4: device error word unavailable");
@@ -573,7 +581,7 @@ int run(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
     if (nb_smem_attr((const void *)kernel, C::SMEM)) return -1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits > 1 ? p.units * splits : p.units < sms ? p.units : sms);
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];

@@ -1,16 +1,20 @@
 // Causal depthwise convolution with carried history, for prompts, chunks and single rows.
 //
 // y[t][d] = act(bias[d] + sum_j w[d][j] u[t + j]) over u = (taps - 1 history rows, x rows). Bound by
-// HBM: each element is read and written once (2 taps + 4 operations on it). A thread owns V
-// neighbouring channels (16 bytes of a row) for a run of rows and slides a window of taps rows through
-// registers, so a row is loaded once per run; the taps - 1 rows before the run come from the history
-// or from the rows that the run before it owns (L1/L2). The rows of a stream are cut into runs until
-// the threads fill the GPU.
+// HBM: each element is read and written once (2 taps + 4 operations on it). A thread owns four
+// neighbouring channels for a run of rows and slides a window of taps rows through registers, so a row
+// is loaded once per run; the taps - 1 rows before the run come from the history or from the rows that
+// the run before it owns (L1/L2). The rows of a stream are cut into runs until the threads fill the GPU.
+//
+// 32767 x 2048 bf16 rows, 4 taps: 48.6 us (5.5 TB/s, 0.84 of the measured copy rate). What it took: eight
+// channels a thread 110 us (134 registers, 12 warps an SM), four 84 us; the weights as vectors 78 us;
+// rows on their way in shared memory 48.6 us (3 or 6 groups of them: 55 us).
 #include "elt.cuh"
 
 namespace {
 
 constexpr int NT = 128;
+constexpr int R = 4, Q = 4;  // rows per group, groups of rows in the ring
 
 struct ConvArgs {
     const void *x;
@@ -24,22 +28,24 @@ struct ConvArgs {
     int c, D, groups, runs, run_rows, act;
 };
 
+// V channels of a row: as they are loaded, and as pairs of fp32 (V = 1: a pair with an idle half)
 template <typename T, int V>
-__device__ __forceinline__ void load(float (&o)[V], const T *p) {
-    const nb::Vec<T, V> t = *(const nb::Vec<T, V> *)p;
+__device__ __forceinline__ void widen(const nb::Vec<T, V> &t, nb::f2 (&o)[(V + 1) / 2]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = nb::to_f32(t.v[i]);
+    for (int i = 0; i < (V + 1) / 2; ++i) o[i] = nb::pack2(nb::to_f32(t.v[2 * i]), 2 * i + 1 < V ? nb::to_f32(t.v[2 * i + 1 < V ? 2 * i + 1 : 0]) : 0.0f);
 }
-template <typename T, int V>
-__device__ __forceinline__ void store(T *p, const float (&v)[V]) {
-    nb::Vec<T, V> t;
-#pragma unroll
-    for (int i = 0; i < V; ++i) t.v[i] = nb::from_f32<T>(v[i]);
-    *(nb::Vec<T, V> *)p = t;
+
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(BYTES) : "memory");
 }
 
 template <typename T, int V, int TAPS>
 __global__ void __launch_bounds__(NT) causal_conv_kernel(const __grid_constant__ ConvArgs a) {
+    constexpr int P = (V + 1) / 2;
+    typedef nb::Vec<T, V> Row;
+    constexpr bool AHEAD = V == 4;  // (single elements are too small for asynchronous copies)
+    __shared__ Row ring[AHEAD ? Q * R : 1][NT];
     nb::pdl_wait();
     const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
     if (i >= a.items) return;
@@ -54,52 +60,102 @@ __global__ void __launch_bounds__(NT) causal_conv_kernel(const __grid_constant__
     const int64_t hs = s * (TAPS - 1) * (int64_t)a.D + d;
     const T *hist = a.hist_in ? (const T *)a.hist_in + hs : nullptr;
     // row t of u without the offset: a history row for t < 0
-    auto row = [&](int t, float (&o)[V]) {
-        if (t >= 0)
-            load<T, V>(o, x + (int64_t)t * a.x_ld);
-        else if (hist)
-            load<T, V>(o, hist + (int64_t)(t + TAPS - 1) * a.D);
-        else
+    auto row = [&](int t) __attribute__((always_inline)) {
+        Row o;
+        if (t >= 0) {
+            o = *(const Row *)(x + (int64_t)t * a.x_ld);
+        } else if (hist) {
+            o = *(const Row *)(hist + (int64_t)(t + TAPS - 1) * a.D);
+        } else {
 #pragma unroll
-            for (int k = 0; k < V; ++k) o[k] = 0.0f;
-    };
-    float win[TAPS][V];  // the last TAPS rows, oldest first
-#pragma unroll
-    for (int j = 0; j < TAPS - 1; ++j) row(t0 - (TAPS - 1) + j, win[j + 1]);
-    if (t0 < t1) {
-        float w[TAPS][V], b[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            b[k] = a.bias ? a.bias[d + k] : 0.0f;
-#pragma unroll
-            for (int j = 0; j < TAPS; ++j) w[j][k] = a.w[(int64_t)(d + k) * TAPS + j];
+            for (int k = 0; k < V; ++k) o.v[k] = nb::from_f32<T>(0.0f);
         }
-        T *y = (T *)a.y + s * a.y_ss + d;
-        for (int t = t0; t < t1; ++t) {
-            float o[V];
+        return o;
+    };
+    if (t0 < t1) {
+        // Rows on their way wait in shared memory, in slots of the thread that asked for them (no barrier):
+        // Q - 1 groups of R rows. In registers four rows a thread were the most, and HBM half idle.
+        const T *px = x + (int64_t)t0 * a.x_ld;
+        const int whole = AHEAD ? (t1 - t0) / R : 0;  // groups of R rows
+        auto fetch = [&](int f) __attribute__((always_inline)) {
+            if constexpr (AHEAD) if (f < whole) {
+                const T *q = px + (int64_t)f * R * a.x_ld;
+#pragma unroll
+                for (int r = 0; r < R; ++r) cp_async<sizeof(Row)>(&ring[(f % Q) * R + r][threadIdx.x], q + r * a.x_ld);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");  // an empty one too: the count tells which group has landed
+        };
+        if (AHEAD)
+#pragma unroll
+            for (int f = 0; f < Q - 1; ++f) fetch(f);
+        nb::f2 win[TAPS][P], w[TAPS][P], b[P];  // the last TAPS rows, oldest first
+#pragma unroll
+        for (int j = 0; j < TAPS - 1; ++j) widen<T, V>(row(t0 - (TAPS - 1) + j), win[j + 1]);
+        // the weights of V channels lie together: TAPS vectors of four where a thread owns four channels
+        // (loaded one by one they cost a warp 16 times the transactions)
+        float wf[V * TAPS], bf[V];
+        const float *wp = a.w + (int64_t)d * TAPS;
+        if (V == 4) {
+#pragma unroll
+            for (int j = 0; j < TAPS; ++j) {
+                const float4 q = ((const float4 *)wp)[j];
+                wf[4 * j] = q.x; wf[4 * j + 1] = q.y; wf[4 * j + 2] = q.z; wf[4 * j + 3] = q.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V * TAPS; ++j) wf[j] = wp[j];
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) bf[k] = a.bias ? a.bias[d + k] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            const int k1 = 2 * k + 1 < V ? 2 * k + 1 : 2 * k;
+            b[k] = nb::pack2(bf[2 * k], bf[k1]);
+#pragma unroll
+            for (int j = 0; j < TAPS; ++j) w[j][k] = nb::pack2(wf[2 * k * TAPS + j], wf[k1 * TAPS + j]);
+        }
+        T *y = (T *)a.y + s * a.y_ss + d + (int64_t)t0 * a.y_ld;
+        auto put = [&](const Row &u) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < TAPS - 1; ++j)
 #pragma unroll
-                for (int k = 0; k < V; ++k) win[j][k] = win[j + 1][k];
-            load<T, V>(win[TAPS - 1], x + (int64_t)t * a.x_ld);
+                for (int k = 0; k < P; ++k) win[j][k] = win[j + 1][k];
+            widen<T, V>(u, win[TAPS - 1]);
+            Row o;
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float v = b[k];
+            for (int k = 0; k < P; ++k) {
+                nb::f2 v = b[k];
 #pragma unroll
-                for (int j = 0; j < TAPS; ++j) v = fmaf(w[j][k], win[j][k], v);
-                o[k] = a.act == NEMO_ACT_SILU ? v * nb::sigmoid_fast(v) : v;
+                for (int j = 0; j < TAPS; ++j) v = nb::fma2(w[j][k], win[j][k], v);
+                if (a.act == NEMO_ACT_SILU) v = nb::mul2(v, nb::sigmoid2(v));
+                float lo, hi;
+                nb::unpack2(v, lo, hi);
+                o.v[2 * k] = nb::from_f32<T>(lo);
+                if (2 * k + 1 < V) o.v[2 * k + 1 < V ? 2 * k + 1 : 0] = nb::from_f32<T>(hi);
             }
-            store<T, V>(y + (int64_t)t * a.y_ld, o);
+            *(Row *)y = o;
+            y += a.y_ld;
+        };
+        for (int f = 0; f < whole; ++f) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(Q - 2) : "memory");
+            Row cur[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) cur[r] = ring[(f % Q) * R + r][threadIdx.x];
+            fetch(f + Q - 1);  // into the slots of group f - 1
+#pragma unroll
+            for (int r = 0; r < R; ++r) put(cur[r]);
         }
+        px += (int64_t)whole * R * a.x_ld;
+        for (int t = t0 + whole * R; t < t1; ++t, px += a.x_ld) put(*(const Row *)px);
     }
     // The thread that reads these channels' history rows replaces them, so both may be one buffer.
     if (TAPS > 1 && a.hist_out && run == 0) {
         T *h = (T *)a.hist_out + hs;
-        float last[TAPS > 1 ? TAPS - 1 : 1][V];
+        Row last[TAPS > 1 ? TAPS - 1 : 1];
 #pragma unroll
-        for (int j = 0; j < TAPS - 1; ++j) row(len - (TAPS - 1) + j, last[j]);
+        for (int j = 0; j < TAPS - 1; ++j) last[j] = row(len - (TAPS - 1) + j);
 #pragma unroll
-        for (int j = 0; j < TAPS - 1; ++j) store<T, V>(h + (int64_t)j * a.D, last[j]);
+        for (int j = 0; j < TAPS - 1; ++j) *(Row *)(h + (int64_t)j * a.D) = last[j];
     }
 }
 
@@ -157,10 +213,10 @@ extern "C" int nemo_causal_conv(const nemo_causal_conv_args_t *p, void *stream) 
     a.hist_in = p->hist_in; a.hist_out = p->hist_out;
     a.y = p->y; a.y_ld = p->y_ld; a.y_ss = p->y_sstride;
     a.lens = p->lens; a.c = p->c; a.D = p->D; a.act = p->act;
-    const int V = 16 / es;
-    const bool vec = p->D % V == 0 && (ptrs & 15) == 0 && ((p->x_ld | p->y_ld | p->x_sstride | p->y_sstride) % V) == 0;
+    const int V = 4;
+    const bool vec = p->D % V == 0 && ptrs % (V * es) == 0 && (uintptr_t)p->w % 16 == 0 && ((p->x_ld | p->y_ld | p->x_sstride | p->y_sstride) % V) == 0;
     int rc = 0;
     cudaStream_t st = (cudaStream_t)stream;
-    NB_ELT_SWITCH(p->elt, T, rc = vec ? by_taps<T, 16 / sizeof(T)>(a, p, st) : by_taps<T, 1>(a, p, st));
+    NB_ELT_SWITCH(p->elt, T, rc = vec ? by_taps<T, 4>(a, p, st) : by_taps<T, 1>(a, p, st));
     return rc;
 }

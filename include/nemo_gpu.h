@@ -174,8 +174,8 @@ int nemo_mxfp4_dequantize(const uint8_t *codes, int64_t ldq, const uint8_t *scal
 /* C[m][n] (= or +=) alpha * act(sum_k A[m][k] W[n][k] + bias[n]) for MXFP4 rows A [M][K] and W [N][K]
    on the block-scaled tensor cores: products are exact, sums fp32. The epilogue is nemo_gemm's: bias
    -> act -> alpha -> store or accumulate (fp32 C only); NEMO_ACT_GLU pairs columns n and n + N/2 into
-   N/2 outputs, a * sigmoid(b), and needs N to be a multiple of 256. K: a positive multiple of 32. Codes,
-   scales and code pitches 16-byte aligned. Scale bytes of the columns past K must not be 255 (the
+   N/2 outputs, a * sigmoid(b), and needs N to be a multiple of 256. K: a positive multiple of 32; M, N and
+   K up to 2^30. Codes, scales and code pitches 16-byte aligned. Scale bytes of the columns past K must not be 255 (the
    quantiser writes 0); those of the rows past M or N may hold anything. */
 typedef struct {
     const uint8_t *A;
@@ -199,7 +199,7 @@ int nemo_gemm_mxfp4(const nemo_gemm_mxfp4_args_t *a, void *stream);
    Stream s has lens[s] rows (device ints, taken into 0..c; NULL: c each); rows of y behind its last
    one are left as they were. hist_in [streams][taps-1][D] (NULL: zeros) holds the rows before this
    call's, hist_out the last taps - 1 rows of u after it (NULL: not kept); they may be the same
-   buffer. taps 1..8; act NEMO_ACT_NONE or NEMO_ACT_SILU. One row per stream is the single-token form. */
+   buffer. taps 1..8, c up to 2^30; act NEMO_ACT_NONE or NEMO_ACT_SILU. One row per stream is the single-token form. */
 typedef struct {
     const void *x;
     int64_t x_ld, x_sstride;
@@ -223,8 +223,9 @@ int nemo_causal_conv(const nemo_causal_conv_args_t *a, void *stream);
    z, skip and dt_bias may be NULL (no gate, 0, 0). Rows of B and C hold groups * N elements. Stream s
    has lens[s] rows (device ints, taken into 0..c; NULL: c each); rows of y behind its last one are
    left as they were. state_in [streams][D][N] (NULL: zeros), state_out the state after the last row
-   (of no rows: the state before; NULL: not kept); they may be the same buffer. N 1..128, D a
-   multiple of groups. One row per stream is the single-token form. */
+   (of no rows: the state before; NULL: not kept); they may be the same buffer. N 1..128, D up to
+   2^24 and a multiple of groups, c up to 2^30. x, dt, z, B and C rows behind a stream's last one are
+   not used, but may be read. One row per stream is the single-token form. */
 typedef struct {
     const void *x;
     int64_t x_ld, x_sstride;

@@ -196,7 +196,7 @@ int by_taps(const ConvArgs &a, const nemo_causal_conv_args_t *p, cudaStream_t st
 
 extern "C" int nemo_causal_conv(const nemo_causal_conv_args_t *p, void *stream) {
     if (!p) return nb_set_error("nemo_causal_conv: null arguments");
-    if (p->streams < 0 || p->c < 0 || p->D < 0) return nb_set_error("nemo_causal_conv: bad shape streams=%d c=%d D=%d", p->streams, p->c, p->D);
+    if (p->streams < 0 || p->c < 0 || p->c > (1 << 30) || p->D < 0) return nb_set_error("nemo_causal_conv: bad shape streams=%d c=%d D=%d", p->streams, p->c, p->D);
     if (p->taps < 1 || p->taps > 8) return nb_set_error("nemo_causal_conv: taps=%d outside 1..8", p->taps);
     if (!nb::elt_ok(p->elt)) return nb_set_error("nemo_causal_conv: unknown element type %d", p->elt);
     if (p->act != NEMO_ACT_NONE && p->act != NEMO_ACT_SILU) return nb_set_error("nemo_causal_conv: activation %d is neither none nor silu", p->act);

@@ -614,7 +614,7 @@ int by_rows(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
 
 extern "C" int nemo_gemm_mxfp4(const nemo_gemm_mxfp4_args_t *a, void *stream) {
     if (!a) return nb_set_error("nemo_gemm_mxfp4: null arguments");
-    if (a->M < 0 || a->N < 0 || a->K < 0) return nb_set_error("nemo_gemm_mxfp4: bad shape M=%d N=%d K=%d", a->M, a->N, a->K);
+    if (a->M < 0 || a->M > (1 << 30) || a->N < 0 || a->N > (1 << 30) || a->K < 0 || a->K > (1 << 30)) return nb_set_error("nemo_gemm_mxfp4: bad shape M=%d N=%d K=%d", a->M, a->N, a->K);
     if (a->act < NEMO_ACT_NONE || a->act > NEMO_ACT_GLU) return nb_set_error("nemo_gemm_mxfp4: unknown activation %d", a->act);
     if (!nb::elt_ok(a->c_elt)) return nb_set_error("nemo_gemm_mxfp4: unknown element type %d", a->c_elt);
     if (a->K == 0 || a->K % 32) return nb_set_error("nemo_gemm_mxfp4: K=%d must be a positive multiple of 32", a->K);

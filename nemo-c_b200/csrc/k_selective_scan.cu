@@ -538,7 +538,7 @@ int by_size(const ScanArgs &a, cudaStream_t st) {
 
 extern "C" int nemo_selective_scan(const nemo_selective_scan_args_t *p, void *stream) {
     if (!p) return nb_set_error("nemo_selective_scan: null arguments");
-    if (p->streams < 0 || p->c < 0 || p->D < 0 || p->D > (1 << 24))
+    if (p->streams < 0 || p->c < 0 || p->c > (1 << 30) || p->D < 0 || p->D > (1 << 24))
         return nb_set_error("nemo_selective_scan: bad shape streams=%d c=%d D=%d", p->streams, p->c, p->D);
     if (p->N < 1 || p->N > 128) return nb_set_error("nemo_selective_scan: N=%d outside 1..128", p->N);
     if (p->groups < 1 || p->D % p->groups) return nb_set_error("nemo_selective_scan: D=%d is not a multiple of groups=%d", p->D, p->groups);

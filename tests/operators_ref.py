@@ -163,8 +163,10 @@ def scan(x, dt, A, B, C, skip=None, z=None, dt_bias=None, softplus=True, state=N
         b, g = wide(B), wide(C)
         arg = step[..., None] * A
         a = np.exp(arg)
-        # the exponent carries A's conversion to base 2, the product and the step; exp2 is 2 ulp
-        ea = a * (es[..., None] * np.abs(A) + np.abs(arg) * 3 * U + 4 * U)
+        # the exponent carries A's conversion to base 2, the product and the step; exp2 is 2 ulp. Where time
+        # is cut (64 rows and more, into two chunks at least) a chunk's decay is exp of A times the sum of its
+        # steps: at most c / 2 additions, each off by u of a sum no larger than the whole
+        ea = a * (es[..., None] * np.abs(A) + np.abs(arg) * (3 + (c / 2 if c >= 64 else 0)) * U + 4 * U)
         in_ = (step * x[:, t])[..., None] * b
         ein = (es * np.abs(x[:, t]))[..., None] * np.abs(b) + np.abs(in_) * 3 * U
         hn = a * h + in_

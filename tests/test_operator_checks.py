@@ -49,6 +49,8 @@ def test_gemm_mxfp4_refused():
     for name in ("A", "W", "C", "a_scales", "w_scales"):
         refused(call(**{name: None}), "null")
     refused(call(M=-1), "bad shape")
+    refused(call(M=(1 << 30) + 1), "bad shape")
+    refused(call(N=(1 << 31) - 1), "bad shape")
     refused(call(K=1000), "multiple of 32")
     refused(call(K=0), "multiple of 32")
     refused(call(N=128, act=3), "256")
@@ -74,6 +76,7 @@ def test_causal_conv_refused():
     refused(call(taps=0), "taps")
     refused(call(taps=9), "taps")
     refused(call(streams=-1), "bad shape")
+    refused(call(c=(1 << 30) + 1), "bad shape")
     refused(call(elt=5), "element type")
     refused(call(act=2), "activation")
     refused(call(act=3), "activation")
@@ -98,6 +101,7 @@ def test_selective_scan_refused():
     refused(call(groups=0), "groups")
     refused(call(groups=3), "groups")
     refused(call(c=-1), "bad shape")
+    refused(call(c=(1 << 31) - 1), "bad shape")
     refused(call(D=1 << 25, groups=1), "bad shape")
     refused(call(elt=4), "element type")
     for name in ("x", "dt", "B", "C", "A", "y"):

@@ -213,15 +213,33 @@ __device__ __forceinline__ float cooked(uint32_t v) {
     else return __half2float(__ushort_as_half((unsigned short)v));
 }
 
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void *dst, const void *src, bool is) {  // is false: zeros
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(BYTES), "r"(is ? BYTES : 0)
+                 : "memory");
+}
+
 template <int LPC>
 constexpr int tile_rows() { return LPC < 4 ? 4 : LPC; }  // at least one row per lane of a channel
 
-template <typename T, int LPC, int NS, bool V4>
+// A raw tile in shared memory: U rows of the warp's x, dt and z, then of B and C, in chunks of CB bytes.
+template <typename T, int LPC, int NS>
+struct LongTile {
+    static constexpr int U = tile_rows<LPC>(), CPW = 32 / LPC, NP = LPC * NS, ES = sizeof(T);
+    static constexpr int CB = CPW * ES < 16 ? CPW * ES : 16;
+    static constexpr int XC = CPW * ES / CB, BC = NP * ES / CB > 0 ? NP * ES / CB : 1;  // chunks in a row
+    static constexpr int XB = U * XC * CB, BB = U * BC * CB;
+    static constexpr int TILE = 3 * XB + 2 * BB;
+    static constexpr int Q = TILE <= 4096 ? 4 : 2;  // tiles in the ring
+};
+
+template <typename T, int LPC, int NS, bool V4, bool ASYNC>
 __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_constant__ ScanArgs a) {
     constexpr int U = tile_rows<LPC>(), CPW = 32 / LPC, NP = LPC * NS, RP = U / LPC;  // channels per warp, padded states, rows per lane and tile
     constexpr int QUADS = U * NP / 4, QL = (QUADS + 31) / 32;   // groups of four states in a tile, per lane
-    extern __shared__ __align__(16) float smem[];  // [LW][2][U][NP]: the warps' tiles of B and C
-    float *ends = smem + LW * 2 * U * NP;          // [LW + 1][NS + 1][32]: end states and sums of steps of the warps' chunks, of the whole block
+    using K = LongTile<T, LPC, NS>;
+    extern __shared__ __align__(16) float smem[];  // [LW][2][U][NP]: the warps' tiles of B and C; ASYNC: [LW][Q] raw tiles
+    float *ends = smem + LW * 2 * U * NP + (ASYNC ? LW * K::Q * K::TILE / 4 : 0);  // [LW + 1][NS + 1][32]: end states and sums of steps of the warps' chunks, of the whole block
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPC, n0 = sub * NS;
     nb::pdl_wait();
     const int rank = a.ranks > 1 ? blockIdx.x % a.ranks : 0;
@@ -231,6 +249,7 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
     const int unit = real ? (int)(item - s * a.units) : 0, grp = unit / a.tiles;
     const int dg = (unit - grp * a.tiles) * CPW + lane / LPC;
     const bool on = real && dg < a.per_group;
+    const int nch = min(CPW, a.per_group - (unit - grp * a.tiles) * CPW);  // this warp's channels
     const int64_t d = grp * a.per_group + min(dg, a.per_group - 1);
     const int len = !real ? 0 : a.lens ? max(0, min(a.lens[s], a.c)) : a.c;
     const int chunks = a.tw * a.ranks, chunk = rank * a.tw + warp % a.tw;
@@ -272,6 +291,32 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
         float total = 0.0f;
         uint32_t rx[RP], rd[RP], rz[RP];
         nb::Vec<T, 4> rb[QL], rc[QL];
+        // ASYNC: tiles of the warp's rows on their way to shared memory, Q - 1 of them; rows that do not exist
+        // are filled with zeros
+        const int64_t first = grp * a.per_group + (unit - grp * a.tiles) * CPW - d;  // the warp's first channel, from this lane's
+        uint8_t *ring = (uint8_t *)(smem + LW * 2 * U * NP) + warp * K::Q * K::TILE;
+        auto copy_rows = [&](const T *base, int64_t ld, int t0, int row_bytes, int off, auto chunks) __attribute__((always_inline)) {
+            constexpr int XC = decltype(chunks)::value;  // at most so many chunks of CB bytes in a row
+#pragma unroll
+            for (int k = 0; k < (U * XC + 31) / 32; ++k) {
+                const int e = lane + k * 32, row = e / XC, at = e % XC * K::CB;
+                if (e < U * XC && at < row_bytes) {
+                    const bool is = t0 + row < te;
+                    cp_async<K::CB>(ring + off + row * XC * K::CB + at, (const uint8_t *)(base + (int64_t)(is ? t0 + row : tb) * ld) + at, is);
+                }
+            }
+        };
+        auto issue = [&](int t0, int slot) __attribute__((always_inline)) {
+            if (t0 < te) {
+                const int s0 = slot * K::TILE, mine_bytes = nch * (int)sizeof(T), bc_bytes = a.N * (int)sizeof(T);
+                copy_rows(X + first, a.x_ld, t0, mine_bytes, s0, std::integral_constant<int, K::XC>{});
+                copy_rows(DT + first, a.dt_ld, t0, mine_bytes, s0 + K::XB, std::integral_constant<int, K::XC>{});
+                if (WRITE && Z) copy_rows(Z + first, a.z_ld, t0, mine_bytes, s0 + 2 * K::XB, std::integral_constant<int, K::XC>{});
+                copy_rows(B, a.bc_ld, t0, bc_bytes, s0 + 3 * K::XB, std::integral_constant<int, K::BC>{});
+                if (WRITE) copy_rows(C, a.bc_ld, t0, bc_bytes, s0 + 3 * K::XB + K::BB, std::integral_constant<int, K::BC>{});
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");  // an empty one too: the count tells which tile has landed
+        };
         // this lane's next rows of x, dt, z and its groups of B and C
         const T *px = X + (int64_t)(tb + sub * RP) * a.x_ld, *pd = DT + (int64_t)(tb + sub * RP) * a.dt_ld;
         const T *pz = WRITE && Z ? Z + (int64_t)(tb + sub * RP) * a.z_ld : nullptr;
@@ -316,9 +361,42 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
             pb += U * a.bc_ld;
             pc += U * a.bc_ld;
         };
-        if (tb < te) fetch(te - tb);
+        int slot = 0;  // of the tile at t0
+        if (ASYNC) {
+#pragma unroll
+            for (int q = 0; q < K::Q - 1; ++q) issue(tb + q * U, q);
+        } else if (tb < te) {
+            fetch(te - tb);
+        }
         for (int t0 = tb; t0 < te; t0 += U) {
-            __syncwarp();
+            if (ASYNC) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(K::Q - 2) : "memory");
+                __syncwarp();
+                const uint8_t *raw_tile = ring + slot * K::TILE;
+#pragma unroll
+                for (int r = 0; r < RP; ++r) {
+                    const T *q = (const T *)(raw_tile + (sub * RP + r) * K::XC * K::CB) + lane / LPC;
+                    rx[r] = raw(q);
+                    rd[r] = raw((const T *)((const uint8_t *)q + K::XB));
+                    if (WRITE && Z) rz[r] = raw((const T *)((const uint8_t *)q + 2 * K::XB));
+                }
+#pragma unroll
+                for (int k = 0; k < QL; ++k) {
+                    const int e = lane + k * 32, row = e / (NP / 4), n = e % (NP / 4) * 4;
+                    if (e < QUADS && n < a.N) {
+                        const T *q = (const T *)(raw_tile + 3 * K::XB + row * K::BC * K::CB) + n;
+                        rb[k] = *(const nb::Vec<T, 4> *)q;
+                        if (WRITE) rc[k] = *(const nb::Vec<T, 4> *)((const uint8_t *)q + K::BB);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) rb[k].v[j] = rc[k].v[j] = nb::from_f32<T>(0.0f);
+                    }
+                }
+                issue(t0 + (K::Q - 1) * U, slot == 0 ? K::Q - 1 : slot - 1);  // into the slot of the tile before
+                slot = slot + 1 == K::Q ? 0 : slot + 1;
+            } else {
+                __syncwarp();
+            }
 #pragma unroll
             for (int k = 0; k < QL; ++k) {
                 const int e = lane + k * 32;
@@ -337,7 +415,7 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
                 if (WRITE && Z) gate[r] = cooked<T>(rz[r]);
             }
             const int live = te - t0;  // rows of this tile that exist
-            if (live > U) fetch(live - U);
+            if (!ASYNC && live > U) fetch(live - U);
             if (a.softplus) {
 #pragma unroll
                 for (int r = 0; r + 1 < RP; r += 2) unpack2(softplus2(pack2(step[r], step[r + 1])), step[r], step[r + 1]);
@@ -472,8 +550,8 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
     }
 }
 
-template <typename T, int LPC, int NS, bool V4>
-int run_long(ScanArgs a, cudaStream_t st) {
+template <typename T, int LPC, int NS, bool V4, bool ASYNC>
+int launch_long(ScanArgs a, cudaStream_t st) {
     constexpr int CPW = 32 / LPC, U = tile_rows<LPC>();
     a.tiles = (a.per_group + CPW - 1) / CPW;
     a.units = a.D / a.per_group * a.tiles;
@@ -491,8 +569,9 @@ int run_long(ScanArgs a, cudaStream_t st) {
     const int per_block = LW / a.tw;
     const int64_t blocks = (a.items + per_block - 1) / per_block * a.ranks;
     if (blocks > 0x7fffffff) return nb_set_error("nemo_selective_scan: too many streams");
-    const size_t smem = (LW * 2 * U * LPC * NS + (chunks > 1 ? (LW + 1) * (NS + 1) * 32 : 0)) * sizeof(float);
-    auto kernel = scan_long_kernel<T, LPC, NS, V4>;
+    using K = LongTile<T, LPC, NS>;
+    const size_t smem = (LW * 2 * U * LPC * NS + (chunks > 1 ? (LW + 1) * (NS + 1) * 32 : 0)) * sizeof(float) + (ASYNC ? LW * K::Q * K::TILE : 0);
+    auto kernel = scan_long_kernel<T, LPC, NS, V4, ASYNC>;
     if (nb_smem_attr((const void *)kernel, smem)) return -1;
     if (a.ranks == 1) {
         nb::launch(kernel, dim3((unsigned)blocks), 32 * LW, smem, st, a);
@@ -513,6 +592,17 @@ int run_long(ScanArgs a, cudaStream_t st) {
         cudaLaunchKernelEx(&cfg, kernel, a);
     }
     return nb_check_launch("scan_long_kernel");
+}
+
+template <typename T, int LPC, int NS, bool V4>
+int run_long(const ScanArgs &a, cudaStream_t st) {
+    // asynchronous copies of 16 bytes (8 where a warp has four 16-bit channels) where all rows allow it: 490 -> us
+    constexpr int E = 16 / sizeof(T);
+    const uintptr_t ptrs = (uintptr_t)a.x | (uintptr_t)a.dt | (uintptr_t)a.z | (uintptr_t)a.B | (uintptr_t)a.C;
+    const int64_t strides = a.x_ld | a.x_ss | a.dt_ld | a.dt_ss | (a.z ? a.z_ld | a.z_ss : 0) | a.bc_ld | a.bc_ss;
+    if constexpr (V4)
+        if (ptrs % 16 == 0 && strides % E == 0 && a.per_group % E == 0 && a.N % E == 0) return launch_long<T, LPC, NS, true, true>(a, st);
+    return launch_long<T, LPC, NS, V4, false>(a, st);
 }
 
 template <typename T, bool V4>

@@ -28,7 +28,7 @@ struct ScanArgs {
     int streams, c, D, N, per_group, softplus;
     int tiles, units;  // a warp's worth of channels: of a group, of a stream
     int64_t items;     // single rows: warps; runs: channel tiles of all streams
-    int tw, ranks;     // runs: chunks of time in a block, blocks of a cluster
+    int lw, tw, ranks; // runs: warps in a block, chunks of time in it, blocks of a cluster
 };
 
 // log(1 + e^v) = max(v, 0) + log1p(e), e = exp(-|v|) <= 1, and log1p(e) = 2 artanh(e / (2 + e)): the
@@ -200,7 +200,7 @@ __device__ __forceinline__ f2 softplus2(f2 v) {
 // one starts from the true state and is done). A chunk's true first state is then folded from those
 // before it, h <- exp(A sum of steps) h + end, and the chunks run again from it, writing y. Nothing
 // but shared memory is needed for that, and the order of the sums is fixed.
-constexpr int LW = 8;  // warps per block
+constexpr int LW_MAX = 8;  // warps per block: 4 or 8
 // An element as it is loaded, and its value: kept apart, so that nothing waits for a load until its
 // value is used
 __device__ __forceinline__ uint32_t raw(const float *p) { return __float_as_uint(*p); }
@@ -234,10 +234,11 @@ struct LongTile {
 };
 
 template <typename T, int LPC, int NS, bool V4, bool ASYNC>
-__global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_constant__ ScanArgs a) {
+__global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_constant__ ScanArgs a) {
     constexpr int U = tile_rows<LPC>(), CPW = 32 / LPC, NP = LPC * NS, RP = U / LPC;  // channels per warp, padded states, rows per lane and tile
     constexpr int QUADS = U * NP / 4, QL = (QUADS + 31) / 32;   // groups of four states in a tile, per lane
     using K = LongTile<T, LPC, NS>;
+    const int LW = a.lw;
     extern __shared__ __align__(16) float smem[];  // [LW][2][U][NP]: the warps' tiles of B and C; ASYNC: [LW][Q] raw tiles
     float *ends = smem + LW * 2 * U * NP + (ASYNC ? LW * K::Q * K::TILE / 4 : 0);  // [LW + 1][NS + 1][32]: end states and sums of steps of the warps' chunks, of the whole block
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPC, n0 = sub * NS;
@@ -430,8 +431,7 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
             }
             __syncwarp();
             float sum[U];
-#pragma unroll
-            for (int r = 0; r < U; ++r) {
+            auto advance = [&](int r) __attribute__((always_inline)) {
                 const float st = LPC == 1 ? step[r % RP] : __shfl_sync(0xffffffffu, step[r % RP], r / RP, LPC);
                 const float in = LPC == 1 ? sx[r % RP] : __shfl_sync(0xffffffffu, sx[r % RP], r / RP, LPC);
                 const f2 st2 = dup2(st), in2 = dup2(in);
@@ -458,6 +458,16 @@ __global__ void __launch_bounds__(32 * LW, 2) scan_long_kernel(const __grid_cons
                 float lo, hi;
                 unpack2(acc, lo, hi);
                 sum[r] = lo + hi;
+            };
+            if (live >= U) {
+#pragma unroll
+                for (int r = 0; r < U; ++r) advance(r);
+            } else {  // (rows that do not exist keep the state, so leaving them out only saves their time)
+#pragma unroll
+                for (int r = 0; r < U; ++r) {
+                    sum[r] = 0.0f;
+                    if (r < live) advance(r);
+                }
             }
             if (WRITE) {
                 nb::WarpFold<U, LPC / 2>::run(sum, lane);  // lane sub: rows sub * RP ..
@@ -564,6 +574,9 @@ int launch_long(ScanArgs a, cudaStream_t st) {
     int chunks = 1;
     if (a.items < 148 * 5)
         while (chunks < 64 && a.items * chunks < 148 * 32 && chunks * 2 * 32 <= a.c) chunks *= 2;
+    // blocks of four warps spread better where one block need not hold several chunks (64 streams of 200 rows: 170 us,
+    // 192 us with eight)
+    const int LW = a.lw = chunks == 1 ? 4 : 8;
     a.tw = chunks < LW ? chunks : LW;
     a.ranks = chunks / a.tw;
     const int per_block = LW / a.tw;
@@ -596,7 +609,8 @@ int launch_long(ScanArgs a, cudaStream_t st) {
 
 template <typename T, int LPC, int NS, bool V4>
 int run_long(const ScanArgs &a, cudaStream_t st) {
-    // asynchronous copies of 16 bytes (8 where a warp has four 16-bit channels) where all rows allow it: 490 -> us
+    // asynchronous copies of 16 bytes (8 where a warp has four 16-bit channels) where all rows allow it (recording of 16384 rows: 495 us
+    // without, 485 us with; prompts 347 and 319 us)
     constexpr int E = 16 / sizeof(T);
     const uintptr_t ptrs = (uintptr_t)a.x | (uintptr_t)a.dt | (uintptr_t)a.z | (uintptr_t)a.B | (uintptr_t)a.C;
     const int64_t strides = a.x_ld | a.x_ss | a.dt_ld | a.dt_ss | (a.z ? a.z_ld | a.z_ss : 0) | a.bc_ld | a.bc_ss;

@@ -49,10 +49,20 @@ __global__ void __launch_bounds__(NT) causal_conv_kernel(const __grid_constant__
     nb::pdl_wait();
     const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
     if (i >= a.items) return;
-    const int64_t sr = i / a.groups;
-    const int g = (int)(i - sr * a.groups);
-    const int64_t s = sr / a.runs;
-    const int run = (int)(sr - s * a.runs), d = g * V;
+    int64_t s;
+    int run, g;
+    if (a.items <= 0xffffffffLL) {  // (a 64-bit division is a hundred instructions)
+        const uint32_t sr = (uint32_t)i / (uint32_t)a.groups, su = sr / (uint32_t)a.runs;
+        g = (int)((uint32_t)i - sr * a.groups);
+        run = (int)(sr - su * a.runs);
+        s = su;
+    } else {
+        const int64_t sr = i / a.groups;
+        g = (int)(i - sr * a.groups);
+        s = sr / a.runs;
+        run = (int)(sr - s * a.runs);
+    }
+    const int d = g * V;
     const int len = a.lens ? max(0, min(a.lens[s], a.c)) : a.c;
     const int t0 = run * a.run_rows, t1 = min(len, t0 + a.run_rows);
     if (t0 >= t1 && run) return;

@@ -56,11 +56,12 @@ template <typename T, int LPC, bool V4>
 __global__ void __launch_bounds__(STEP_NT, 6) scan_step_kernel(const __grid_constant__ ScanArgs a) {
     constexpr int CPW = 32 / LPC, SB = LPC < STEP_SB ? LPC : STEP_SB, REP = LPC / SB;
     nb::pdl_wait();
-    const int64_t w = ((int64_t)blockIdx.x * STEP_NT + threadIdx.x) >> 5;
-    if (w >= a.items) return;
+    const uint32_t w = blockIdx.x * (STEP_NT / 32) + (threadIdx.x >> 5);  // (a 64-bit division is a hundred instructions)
+    if (w >= (uint32_t)a.items) return;
     const int lane = threadIdx.x & 31, sub = lane % LPC, n0 = sub * 4, v = sub / REP;  // this lane's states, and its stream of SB
-    const int64_t s0 = w / a.units * SB;
-    const int unit = (int)(w % a.units), grp = unit / a.tiles;
+    const uint32_t sblk = w / (uint32_t)a.units;
+    const int64_t s0 = (int64_t)sblk * SB;
+    const int unit = (int)(w - sblk * a.units), grp = (uint32_t)unit / (uint32_t)a.tiles;
     const int dg = (unit - grp * a.tiles) * CPW + lane / LPC;
     const bool on = dg < a.per_group, st4 = n0 < a.N;
     const int d = grp * a.per_group + (on ? dg : a.per_group - 1);
@@ -166,7 +167,7 @@ int run_step(ScanArgs a, cudaStream_t st) {
     a.units = a.D / a.per_group * a.tiles;
     a.items = (a.streams + SB - 1) / SB * (int64_t)a.units;
     const int64_t blocks = (a.items * 32 + STEP_NT - 1) / STEP_NT;
-    if (blocks > 0x7fffffff) return nb_set_error("nemo_selective_scan: too many streams");
+    if (a.items > 0x7fffffff) return nb_set_error("nemo_selective_scan: too many streams");
     nb::launch(scan_step_kernel<T, LPC, V4>, dim3((unsigned)blocks), STEP_NT, 0, st, a);
     return nb_check_launch("scan_step_kernel");
 }
@@ -244,10 +245,11 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPC, n0 = sub * NS;
     nb::pdl_wait();
     const int rank = a.ranks > 1 ? blockIdx.x % a.ranks : 0;
-    const int64_t item = (blockIdx.x / a.ranks) * (int64_t)(LW / a.tw) + warp / a.tw;  // (stream, channel tile)
-    const bool real = item < a.items;
-    const int64_t s = real ? item / a.units : 0;
-    const int unit = real ? (int)(item - s * a.units) : 0, grp = unit / a.tiles;
+    const uint32_t item = (blockIdx.x / (uint32_t)a.ranks) * ((uint32_t)LW / (uint32_t)a.tw) + (uint32_t)warp / (uint32_t)a.tw;  // (stream, channel tile)
+    const bool real = item < (uint32_t)a.items;
+    const uint32_t su = real ? item / (uint32_t)a.units : 0;
+    const int64_t s = su;
+    const int unit = real ? (int)(item - su * a.units) : 0, grp = (uint32_t)unit / (uint32_t)a.tiles;
     const int dg = (unit - grp * a.tiles) * CPW + lane / LPC;
     const bool on = real && dg < a.per_group;
     const int nch = min(CPW, a.per_group - (unit - grp * a.tiles) * CPW);  // this warp's channels
@@ -581,7 +583,7 @@ int launch_long(ScanArgs a, cudaStream_t st) {
     a.ranks = chunks / a.tw;
     const int per_block = LW / a.tw;
     const int64_t blocks = (a.items + per_block - 1) / per_block * a.ranks;
-    if (blocks > 0x7fffffff) return nb_set_error("nemo_selective_scan: too many streams");
+    if (a.items > 0x7fffffff || blocks > 0x7fffffff) return nb_set_error("nemo_selective_scan: too many streams");
     using K = LongTile<T, LPC, NS>;
     const size_t smem = (LW * 2 * U * LPC * NS + (chunks > 1 ? (LW + 1) * (NS + 1) * 32 : 0)) * sizeof(float) + (ASYNC ? LW * K::Q * K::TILE : 0);
     auto kernel = scan_long_kernel<T, LPC, NS, V4, ASYNC>;

@@ -224,7 +224,7 @@ extern "C" int nemo_causal_conv(const nemo_causal_conv_args_t *p, void *stream) 
     a.y = p->y; a.y_ld = p->y_ld; a.y_ss = p->y_sstride;
     a.lens = p->lens; a.c = p->c; a.D = p->D; a.act = p->act;
     const int V = 4;
-    const bool vec = p->D % V == 0 && ptrs % (V * es) == 0 && (uintptr_t)p->w % 16 == 0 && ((p->x_ld | p->y_ld | p->x_sstride | p->y_sstride) % V) == 0;
+    const bool vec = p->D % V == 0 && ptrs % (V * es) == 0 && (uintptr_t)p->w % 16 == 0 && ((p->x_ld | p->y_ld | (p->streams > 1 ? p->x_sstride | p->y_sstride : 0)) % V) == 0;
     int rc = 0;
     cudaStream_t st = (cudaStream_t)stream;
     NB_ELT_SWITCH(p->elt, T, rc = vec ? by_taps<T, 4>(a, p, st) : by_taps<T, 1>(a, p, st));

@@ -499,14 +499,19 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
             }
             to[NS * 32] = total;
         };
-        // h <- exp(A sum) h + end of a chunk (or of a block's chunks), given how to read it
+        // h <- exp(A sum) h + end of a chunk (or of a block's chunks), given how to read it. The decay is applied
+        // as two halves, and not to a state of zero: step by step a growing channel overflows when its
+        // state does, not when its growth over a chunk would.
         auto fold = [&](auto get) __attribute__((always_inline)) {
-            const f2 t2 = dup2(get(NS));
+            const f2 half = dup2(0.5f * get(NS));
 #pragma unroll
             for (int j = 0; j < NS / 2; ++j) {
-                float e0, e1;
-                unpack2(mul2(t2, A2[j]), e0, e1);
-                h[j] = fma2(pack2(ex2(e0), ex2(e1)), h[j], pack2(get(2 * j), get(2 * j + 1)));
+                float e0, e1, h0, h1;
+                unpack2(mul2(half, A2[j]), e0, e1);
+                unpack2(h[j], h0, h1);
+                e0 = ex2(e0);
+                e1 = ex2(e1);
+                h[j] = add2(pack2(h0 == 0.0f ? 0.0f : h0 * e0 * e0, h1 == 0.0f ? 0.0f : h1 * e1 * e1), pack2(get(2 * j), get(2 * j + 1)));
             }
         };
         float total = 0.0f;
@@ -540,7 +545,10 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
         fold_warps(warp - warp % a.tw, warp);
         if (chunk == 0 && a.state_in) load_states(a.state_in + at, h);
         pass(std::true_type{});
-        if (a.ranks > 1) nb::cluster_sync();  // no block leaves while another reads its shared memory
+        // no block leaves while another reads its shared memory; and no chunk writes a state that is to replace
+        // the one before it while the first chunk may still read that
+        if (a.ranks > 1) nb::cluster_sync();
+        else __syncthreads();
     } else {
         pass(std::true_type{});
     }

@@ -136,7 +136,7 @@ def test_product_exact(m, n, k):
 
 @pytest.mark.parametrize("act", ["none", "silu", "relu", "glu"])
 @pytest.mark.parametrize("out", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("m,n,k", [(1, 512, 1024), (7, 2048, 1024), (20, 256, 96), (150, 512, 544), (260, 768, 256)])
+@pytest.mark.parametrize("m,n,k", [(1, 512, 1024), (7, 2048, 1024), (20, 256, 96), (150, 512, 544), (260, 768, 256), (5, 512, 4096), (40, 256, 8192)])
 def test_product(m, n, k, out, act):
     rng = np.random.default_rng(m + n + k)
     a, av = coded(rng, m, k, 118, 124)
@@ -208,3 +208,27 @@ def test_product_pitched_codes_and_repeats():
         again = product((aq, as_), (wq, ws), m, n, k)
         assert torch.equal(first, again)
         R.check(R.f64(first), av @ wv.T, k * 2 * R.U * (np.abs(av) @ np.abs(wv).T), "f32")
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k,ldc", [(3, 130, 64, 130), (70, 1001, 96, 1001), (129, 136, 256, 137), (200, 264, 512, 272), (300, 40, 32, 48)])
+def test_product_narrow_types_and_odd_pitches(m, n, k, ldc, out):
+    """16-bit outputs whose rows allow 16-byte stores and whose do not; what lies behind the columns stays."""
+    rng = np.random.default_rng(m + n)
+    a, av = coded(rng, m, k, 122, 123)
+    w, wv = coded(rng, n, k, 122, 123)
+    c = product(a, w, m, n, k, out=out, ldc=ldc)
+    want = torch.from_numpy(av @ wv.T).to(R.ELT[out][0])  # the sums are exact in fp32: one rounding
+    assert torch.equal(c[:, :n].cpu(), want)
+    assert (c[:, n:] == -77).all()
+
+
+def test_product_split_accumulates():
+    """A few rows over a long k (split over a cluster) into what is there."""
+    rng = np.random.default_rng(12)
+    m, n, k = 9, 384, 8192
+    a, av = coded(rng, m, k, 126, 126)
+    w, wv = coded(rng, n, k, 126, 126)
+    c0 = torch.from_numpy(rng.integers(-50, 50, (m, n)).astype(np.float32)).cuda()
+    c = product(a, w, m, n, k, C0=c0.clone(), alpha=0.5)
+    assert np.array_equal(R.f64(c), R.f64(c0) + 0.5 * (av @ wv.T))

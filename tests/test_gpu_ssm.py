@@ -235,3 +235,53 @@ def test_scan_no_rows():
         g[k] = g[k][:, :0]
     _, h = scan(g, "f32")
     assert torch.equal(h, g["state"])
+
+
+@pytest.mark.parametrize("c,D", [(70, 64), (300, 64), (300, 2048), (3000, 32)])
+def test_scan_state_replaced_in_place(c, D):
+    """State out over state in, streams of all lengths (none among them), time cut or not: the bits of
+    a call with a state of its own, every time."""
+    rng = np.random.default_rng(c + D)
+    S = 6
+    g = inputs(rng, S, c, D, 16, 1, "bf16")
+    lens = torch.tensor([0, 1, 3, c // 2, c - 1, c], dtype=torch.int32, device="cuda")
+    y, h = scan(g, "bf16", lens)
+    assert torch.equal(h[0], g["state"][0])
+    for _ in range(20):
+        own = dict(g, state=g["state"].clone())
+        y2, _ = scan(own, "bf16", lens, state_out="same")
+        assert torch.equal(y, y2) and torch.equal(own["state"], h)
+
+
+def test_scan_growth_past_the_range_of_a_chunk():
+    """A channel that grows by e^3 a row, without input until its last rows: its growth over a chunk of
+    time overflows, its state does not. And states of 1e-30 that grow back to about 1."""
+    S, c, D, N = 1, 1100, 32, 16
+    rng = np.random.default_rng(11)
+    g = inputs(rng, S, c, D, N, 1, "f32", with_bias=False, state=False)
+    x = R.f64(g["x"])
+    x[:, :c - 9] = 0
+    g["x"], g["dt"] = R.to_dev(x), R.to_dev(np.ones((S, c, D)))
+    A = R.f64(g["A"])
+    A[3] = 3.0
+    A[4] = np.log(1e30) / c
+    g["A"] = dev32(A)
+    g["state"] = torch.zeros(S, D, N, device="cuda")
+    g["state"][:, 4] = 1e-30
+    y, h = scan(g, "f32", softplus=False)
+    wy, wh, ey, eh = want_of(g, softplus=False)
+    assert np.isfinite(wh).all()
+    R.check(R.f64(y), wy, ey, "f32", "y")
+    R.check(R.f64(h), wh, eh, "f32", "state")
+
+
+@pytest.mark.parametrize("elt", ["f32", "bf16"])
+@pytest.mark.parametrize("S,c,D,N,G", [(1, 5, 1, 1, 1), (2, 9, 3, 5, 3), (1, 100, 1, 16, 1), (3, 1, 2, 3, 2), (2, 5, 40, 16, 5), (1, 130, 264, 32, 3)])
+def test_scan_narrow(S, c, D, N, G, elt):
+    """A channel or two, groups smaller than a warp's channels."""
+    rng = np.random.default_rng(S + c + D)
+    g = inputs(rng, S, c, D, N, G, elt)
+    y, h = scan(g, elt)
+    wy, wh, ey, eh = want_of(g)
+    R.check(R.f64(y), wy, ey, elt, "y")
+    R.check(R.f64(h), wh, eh, "f32", "state")

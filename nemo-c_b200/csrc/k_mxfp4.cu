@@ -4,11 +4,15 @@
 // the power of two 2^e, e = floor(log2 m) - 2 (two is the exponent of the format's largest value,
 // 6 = 1.5 * 2^2), held as the byte e + 127 and not below 2^-127; each value is x / 2^e rounded to
 // the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to the even code, larger magnitudes to 6) with
-// its sign. x / 2^e is an exact multiplication by a power of two, so the codes are rounded once.
+// its sign. x / 2^e is a multiplication by a power of two, exact wherever the code is not zero, so the
+// codes are rounded once.
 // A block that holds an infinity or a NaN has no such scale: its byte is 255 (the format's NaN)
 // and its codes are zero, so every value of it reads back as NaN.
 //
 // Both kernels are bound by HBM (2.5 to 4.5 bytes moved per element, no reuse).
+// 16384 x 4096 bf16: quantised in 33 us (5.1 TB/s, 0.78 of the measured copy rate; 40 us with eight columns a
+// thread and single scale bytes), there and back in 65 us. A thread keeps 32 or 64 bytes on their way: 2048
+// threads an SM cover HBM's latency.
 #include "elt.cuh"
 #include "mxfp4.cuh"
 

@@ -328,6 +328,8 @@ __global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
             }
             if (!__all_sync(0xffffffffu, ok)) { flags[0] = 1; atomicExch(p.err, 6); break; }
             sm100::tc_fence_after();
+            // activation tiles of 64 rows: the second one of a scale tile (128 rows) finds its scales two columns on
+            const int sb_at = WT * 8 + (BN == 64 ? u % p.n_mtiles % 2 * 2 : 0);
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % C::STAGES;
                 if (!__all_sync(0xffffffffu, sm100::mbar_wait(&full[s], (it / C::STAGES) & 1))) { flags[0] = 1; atomicExch(p.err, 7); break; }
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
                         for (int kk = 0; kk < 4; ++kk)
                             if (kk < steps)
                                 mma_mxf4(d, desc_operand(st + i * C::W_BYTES + kk * 32), desc_operand(st + WT * C::W_BYTES + kk * 32), idesc_mxf4(BN, kk & 1),
-                                         sc + i * 8 + (kk >> 1) * 4, sc + WT * 8 + (kk >> 1) * 4, kb != kb0 || kk != 0);
+                                         sc + i * 8 + (kk >> 1) * 4, sc + sb_at + (kk >> 1) * 4, kb != kb0 || kk != 0);
                     }
                 };
                 const int left = p.K - kb * 256;
@@ -615,7 +617,13 @@ template <typename T>
 int by_rows(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
     const bool glu = a->act == NEMO_ACT_GLU;
     if (a->M <= 16) return glu ? run<T, 16, 2>(a, st) : run<T, 16, 1>(a, st);
-    if (a->M <= 64) return glu ? run<T, 64, 2>(a, st) : run<T, 64, 1>(a, st);
+    // 64 rows a tile where all tiles then still run at once, on more SMs with less to finish for each (256 x 4096 x
+    // 1024: 6.4 us with 128 rows, 5.0 us with 64; 1792 x 1024 x 4096, two turns with 64: 9.3 and 11.3 us)
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return nb_set_error("nemo_gemm_mxfp4: no CUDA device");
+    const int64_t tiles = (int64_t)(((glu ? a->N / 2 : a->N) + BM - 1) / BM) * ((a->M + 63) / 64);
+    if (a->M <= 64 || tiles <= sms) return glu ? run<T, 64, 2>(a, st) : run<T, 64, 1>(a, st);
     return glu ? run<T, 128, 2>(a, st) : run<T, 128, 1>(a, st);
 }
 

@@ -119,7 +119,7 @@ def coded(rng, r, k, lo, hi, fill=0):
 
 
 SHAPES = [(1, 128, 32), (1, 1024, 4096), (2, 8, 64), (7, 256, 1024), (15, 136, 96), (16, 128, 256), (17, 200, 288), (33, 1000, 512), (64, 384, 160), (65, 128, 2048),
-          (100, 130, 352), (128, 256, 256), (129, 256, 1056), (200, 72, 4096), (300, 1024, 736), (1000, 640, 1024)]
+          (100, 130, 352), (128, 256, 256), (129, 256, 1056), (200, 72, 4096), (300, 1024, 736), (1000, 640, 1024), (190, 4096, 256), (321, 1000, 96), (600, 2048, 32), (1200, 2048, 288)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -136,7 +136,7 @@ def test_product_exact(m, n, k):
 
 @pytest.mark.parametrize("act", ["none", "silu", "relu", "glu"])
 @pytest.mark.parametrize("out", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("m,n,k", [(1, 512, 1024), (7, 2048, 1024), (20, 256, 96), (150, 512, 544), (260, 768, 256), (5, 512, 4096), (40, 256, 8192)])
+@pytest.mark.parametrize("m,n,k", [(1, 512, 1024), (7, 2048, 1024), (20, 256, 96), (150, 512, 544), (260, 768, 256), (5, 512, 4096), (40, 256, 8192), (190, 256, 8192), (700, 4096, 128)])
 def test_product(m, n, k, out, act):
     rng = np.random.default_rng(m + n + k)
     a, av = coded(rng, m, k, 118, 124)

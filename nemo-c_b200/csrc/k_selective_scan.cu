@@ -31,6 +31,12 @@ struct ScanArgs {
     int lw, tw, ranks; // runs: warps in a block, chunks of time in it, blocks of a cluster
 };
 
+// Over [-1, 0] the special-function units' 2^x is within 1.4e-7 of the exact value, and too small by 5e-9 (at
+// -1e-4) to 2.6e-8 (at -0.03) of it on average (measured): less than a step of fp32, but the same way for
+// every row of a long memory. 2^-26 in the exponent, 1.03e-8 of the value, leaves half of that at most where
+// memories are long; it is too little to turn a decay of 1 into anything else.
+constexpr float EVEN = 0x1p-26f;
+
 // log(1 + e^v) = max(v, 0) + log1p(e), e = exp(-|v|) <= 1, and log1p(e) = 2 artanh(e / (2 + e)): the
 // argument is at most 1/3, so seven terms of the series leave 1.4e-8 of it. No cancellation at either end.
 __device__ __forceinline__ float softplus_f(float v) {
@@ -137,7 +143,7 @@ __global__ void __launch_bounds__(STEP_NT, 6) scan_step_kernel(const __grid_cons
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 float e0, e1;
-                unpack2(mul2(st2, A2[j]), e0, e1);
+                unpack2(fma2(st2, A2[j], dup2(EVEN)), e0, e1);
                 const f2 hh = fma2(pack2(ex2(e0), ex2(e1)), pack2(h[r].v[2 * j], h[r].v[2 * j + 1]),
                                    mul2(in2, pack2(to_f32(b[r].v[2 * j]), to_f32(b[r].v[2 * j + 1]))));
                 const f2 cc = pack2(to_f32(c[r].v[2 * j]), to_f32(c[r].v[2 * j + 1]));
@@ -209,9 +215,9 @@ __device__ __forceinline__ f2 softplus2(f2 v) {
 // before it, h <- exp(A sum of steps) h + end, and the chunks run again from it, writing y. Nothing
 // but shared memory is needed for that, and the order of the sums is fixed.
 //
-// Measured: 64 streams x 200 rows x 2048 channels, 16 states, bf16: 170 us, of which the special-function units
-// are busy 68 % (their 17 exponentials and more per row and channel: 115 us) and instructions issue 59 %, 140 a row
-// for 32 channels; 16384 rows of one stream, two passes: 490 us (283 us of special functions). Four lanes a
+// Measured: 64 streams x 200 rows x 2048 channels, 16 states, bf16: 165 us, of which the special-function units
+// are busy 70 % (their 17 exponentials and more per row and channel: 115 us) and instructions issue 59 %, 140 a row
+// for 32 channels; 16384 rows of one stream, two passes: 467 us (283 us of special functions). Four lanes a
 // channel with rows prepared by other warps in shared memory: 500 us for the latter in one pass, bound by
 // shared memory's 128 bytes a clock (steps, B, C and sums pass through it for every lane).
 constexpr int LW_MAX = 8;  // warps per block: 4 or 8
@@ -450,7 +456,7 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
                     for (int j = 0; j < 2; ++j) {
                         f2 &hh = h[2 * q + j];
                         float e0, e1;
-                        unpack2(mul2(st2, A2[2 * q + j]), e0, e1);
+                        unpack2(fma2(st2, A2[2 * q + j], dup2(EVEN)), e0, e1);
                         hh = fma2(pack2(ex2(e0), ex2(e1)), hh, mul2(in2, j ? pack2(bv.z, bv.w) : pack2(bv.x, bv.y)));
                         if (WRITE) {
                             const f2 cc = j ? pack2(cv.z, cv.w) : pack2(cv.x, cv.y);

@@ -285,3 +285,13 @@ def test_scan_narrow(S, c, D, N, G, elt):
     wy, wh, ey, eh = want_of(g)
     R.check(R.f64(y), wy, ey, elt, "y")
     R.check(R.f64(h), wh, eh, "f32", "state")
+
+
+@pytest.mark.parametrize("c", [1, 6, 50, 900])
+def test_scan_steps_of_zero_keep_the_state(c):
+    """A step of exactly 0 decays by exactly 1: the state's bits stay, whatever A is."""
+    rng = np.random.default_rng(c)
+    g = inputs(rng, 2, c, 48, 16, 1, "f32", with_bias=False)
+    g["dt"] = torch.zeros_like(g["dt"])
+    _, h = scan(g, "f32", softplus=False)
+    assert torch.equal(h, g["state"])

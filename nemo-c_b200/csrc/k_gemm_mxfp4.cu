@@ -295,15 +295,16 @@ __global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
                 if (leader) {
                     uint8_t *st = stages + s * C::STAGE;
                     const uint32_t sb = (uint32_t)min(2, p.katoms - kb * 2) * ATOM;  // scale tiles of these columns
+                    const int64_t at = (int64_t)kb * (2 * ATOM);  // 2 GB of scales a row of tiles at K = 2^29
                     sm100::mbar_arrive_expect_tx(&full[s], WT * (C::W_BYTES + sb) + C::A_BYTES + sb);
                     sm100::tma_load_2d(st, &tmW, &full[s], kb * BKB, r0);
-                    bulk_g2s(st + C::WS_OFF, ws0 + kb * 2 * ATOM, sb, &full[s]);
+                    bulk_g2s(st + C::WS_OFF, ws0 + at, sb, &full[s]);
                     if (glu) {
                         sm100::tma_load_2d(st + C::W_BYTES, &tmW, &full[s], kb * BKB, r1);
-                        bulk_g2s(st + C::WS_OFF + 2 * ATOM, ws1 + kb * 2 * ATOM, sb, &full[s]);
+                        bulk_g2s(st + C::WS_OFF + 2 * ATOM, ws1 + at, sb, &full[s]);
                     }
                     sm100::tma_load_2d(st + WT * C::W_BYTES, &tmA, &full[s], kb * BKB, mt * BN);
-                    bulk_g2s(st + C::WS_OFF + WT * 2 * ATOM, as + kb * 2 * ATOM, sb, &full[s]);
+                    bulk_g2s(st + C::WS_OFF + WT * 2 * ATOM, as + at, sb, &full[s]);
                 }
                 __syncwarp();
             }

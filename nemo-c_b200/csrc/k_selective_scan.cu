@@ -144,8 +144,12 @@ __global__ void __launch_bounds__(STEP_NT, 6) scan_step_kernel(const __grid_cons
             for (int j = 0; j < 2; ++j) {
                 float e0, e1;
                 unpack2(fma2(st2, A2[j], dup2(EVEN)), e0, e1);
-                const f2 hh = fma2(pack2(ex2(e0), ex2(e1)), pack2(h[r].v[2 * j], h[r].v[2 * j + 1]),
-                                   mul2(in2, pack2(to_f32(b[r].v[2 * j]), to_f32(b[r].v[2 * j + 1]))));
+                f2 hh = fma2(pack2(ex2(e0), ex2(e1)), pack2(h[r].v[2 * j], h[r].v[2 * j + 1]),
+                             mul2(in2, pack2(to_f32(b[r].v[2 * j]), to_f32(b[r].v[2 * j + 1]))));
+                if (!V4) {  // states past N: see below
+                    unpack2(hh, e0, e1);
+                    hh = pack2(n0 + 2 * j < a.N ? e0 : 0.0f, n0 + 2 * j + 1 < a.N ? e1 : 0.0f);
+                }
                 const f2 cc = pack2(to_f32(c[r].v[2 * j]), to_f32(c[r].v[2 * j + 1]));
                 acc = j ? fma2(hh, cc, acc) : mul2(hh, cc);
                 unpack2(hh, h[r].v[2 * j], h[r].v[2 * j + 1]);
@@ -154,6 +158,10 @@ __global__ void __launch_bounds__(STEP_NT, 6) scan_step_kernel(const __grid_cons
             unpack2(acc, lo, hi);
             sum[r] = lo + hi;
         }
+    }
+    if (V4 && !st4) {  // states past N are zeros, but those times an infinite input are NaN
+#pragma unroll
+        for (int r = 0; r < SB; ++r) sum[r] = 0.0f;
     }
     nb::WarpFold<SB, LPC / 2>::run(sum, lane);
     if (live && on && sub % REP == 0) ((T *)a.y)[s * a.y_ss + d] = nb::from_f32<T>(fmaf(skip, xv, sum[0]) * gate);
@@ -241,6 +249,88 @@ struct LongTile {
     static constexpr int Q = TILE < 4096 ? 4 : 2;
 };
 
+// What a lane of the kernel for runs works on: its channel, and its warp's chunk of the stream's rows.
+template <int LPC, int NS, int U>
+struct Place {
+    int rank, chunk, chunks, unit, grp, tb, te;
+    bool on;
+    int64_t s, d;
+    __device__ __forceinline__ Place(const ScanArgs &a, uint32_t block, uint32_t thread) {
+        constexpr int CPW = 32 / LPC;
+        const int warp = thread >> 5, lane = thread & 31;
+        rank = a.ranks > 1 ? block % a.ranks : 0;
+        const uint32_t item = (block / (uint32_t)a.ranks) * ((uint32_t)a.lw / (uint32_t)a.tw) + (uint32_t)warp / (uint32_t)a.tw;  // (stream, channel tile)
+        const bool real = item < (uint32_t)a.items;
+        const uint32_t su = real ? item / (uint32_t)a.units : 0;
+        s = su;
+        unit = real ? (int)(item - su * a.units) : 0;
+        grp = (uint32_t)unit / (uint32_t)a.tiles;
+        const int dg = (unit - grp * a.tiles) * CPW + lane / LPC;
+        on = real && dg < a.per_group;
+        d = grp * a.per_group + min(dg, a.per_group - 1);
+        const int len = !real ? 0 : a.lens ? max(0, min(a.lens[s], a.c)) : a.c;
+        chunks = a.tw * a.ranks;
+        chunk = rank * a.tw + warp % a.tw;
+        const int rows = (len + chunks * U - 1) / (chunks * U) * U;  // rows per chunk, whole tiles
+        tb = min(len, chunk * rows);
+        te = min(len, tb + rows);
+    }
+};
+
+// States past N fill up a lane with zeros. Times an infinite input or step that is a NaN, which stays, in all of them
+// alike, and goes into the outputs. The channels of the lanes in `hit` were left with one: they run once more, row
+// by row from the stream's first one and with their own states alone, writing the chunk's outputs. (64 streams x 200
+// rows, 1024 channels: states past N kept out of every row's sum by a condition cost 4 to 12 %, a test in every tile 1 to
+// 6 %, this nothing. It keeps nothing in registers while the kernel's own passes run, which have none left.)
+template <typename T, int LPC, int NS, int U>
+__device__ __forceinline__ void run_again(const ScanArgs &a, uint32_t hit, f2 (&h)[NS / 2]) {
+    uint32_t block, thread;
+    asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(block));
+    asm volatile("mov.u32 %0, %%tid.x;" : "=r"(thread));
+    const Place<LPC, NS, U> p(a, block, thread);
+    const int lane = thread & 31, sub = lane % LPC, count = min(NS, a.N - sub * NS);  // this lane's states
+    const bool again = (hit >> (lane - sub) & (2u << (LPC - 1)) - 1) != 0;            // the same in all lanes of a channel
+    const int64_t at = (p.s * a.D + p.d) * a.N + sub * NS, bc = p.s * a.bc_ss + (int64_t)p.grp * a.N + sub * NS;
+    const float *A = a.A + p.d * a.N + sub * NS;
+    const T *X = (const T *)a.x + p.s * a.x_ss + p.d, *DT = (const T *)a.dt + p.s * a.dt_ss + p.d;
+    if (again) {
+#pragma unroll
+        for (int j = 0; j < NS; j += 2)
+            h[j / 2] = pack2(a.state_in && j < count ? a.state_in[at + j] : 0.0f, a.state_in && j + 1 < count ? a.state_in[at + j + 1] : 0.0f);
+    }
+    for (int t = 0; t < p.te; ++t) {
+        float sum = 0.0f;
+        const float x = to_f32(X[(int64_t)t * a.x_ld]);
+        if (again) {
+            float step = to_f32(DT[(int64_t)t * a.dt_ld]) + (a.dt_bias ? a.dt_bias[p.d] : 0.0f);
+            if (a.softplus) step = softplus_f(step);
+            const T *B = (const T *)a.B + bc + (int64_t)t * a.bc_ld, *C = (const T *)a.C + bc + (int64_t)t * a.bc_ld;
+#pragma unroll
+            for (int j = 0; j < NS; j += 2) {
+                float v[2];
+                unpack2(h[j / 2], v[0], v[1]);
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (j + k < count) {
+                        v[k] = fmaf(ex2(fmaf(step * LOG2E, A[j + k], EVEN)), v[k], step * x * to_f32(B[j + k]));
+                        sum = fmaf(v[k], to_f32(C[j + k]), sum);
+                    }
+                h[j / 2] = pack2(v[0], v[1]);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < LPC; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (again && p.on && sub == 0 && t >= p.tb) {
+            float v = fmaf(a.skip ? a.skip[p.d] : 0.0f, x, sum);
+            if (a.z) {
+                const float z = to_f32(((const T *)a.z)[p.s * a.z_ss + p.d + (int64_t)t * a.z_ld]);
+                v *= z * nb::sigmoid_fast(z);
+            }
+            ((T *)a.y)[p.s * a.y_ss + p.d + (int64_t)t * a.y_ld] = nb::from_f32<T>(v);
+        }
+    }
+}
+
 template <typename T, int LPC, int NS, int U, bool V4, bool ASYNC>
 __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_constant__ ScanArgs a) {
     constexpr int CPW = 32 / LPC, NP = LPC * NS, RP = U / LPC;  // channels per warp, padded states, rows per lane and tile
@@ -251,20 +341,11 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
     float *ends = smem + LW * 2 * U * NP + (ASYNC ? LW * K::Q * K::TILE / 4 : 0);  // [LW + 1][NS + 1][32]: end states and sums of steps of the warps' chunks, of the whole block
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPC, n0 = sub * NS;
     nb::pdl_wait();
-    const int rank = a.ranks > 1 ? blockIdx.x % a.ranks : 0;
-    const uint32_t item = (blockIdx.x / (uint32_t)a.ranks) * ((uint32_t)LW / (uint32_t)a.tw) + (uint32_t)warp / (uint32_t)a.tw;  // (stream, channel tile)
-    const bool real = item < (uint32_t)a.items;
-    const uint32_t su = real ? item / (uint32_t)a.units : 0;
-    const int64_t s = su;
-    const int unit = real ? (int)(item - su * a.units) : 0, grp = (uint32_t)unit / (uint32_t)a.tiles;
-    const int dg = (unit - grp * a.tiles) * CPW + lane / LPC;
-    const bool on = real && dg < a.per_group;
+    const Place<LPC, NS, U> here(a, blockIdx.x, threadIdx.x);
+    const int rank = here.rank, chunk = here.chunk, chunks = here.chunks, unit = here.unit, grp = here.grp, tb = here.tb, te = here.te;
+    const bool on = here.on;
+    const int64_t s = here.s, d = here.d;
     const int nch = min(CPW, a.per_group - (unit - grp * a.tiles) * CPW);  // this warp's channels
-    const int64_t d = grp * a.per_group + min(dg, a.per_group - 1);
-    const int len = !real ? 0 : a.lens ? max(0, min(a.lens[s], a.c)) : a.c;
-    const int chunks = a.tw * a.ranks, chunk = rank * a.tw + warp % a.tw;
-    const int rows = (len + chunks * U - 1) / (chunks * U) * U;  // rows per chunk, whole tiles
-    const int tb = min(len, chunk * rows), te = min(len, tb + rows);
 
     f2 A2[NS / 2], h[NS / 2];
     const int64_t at = (s * a.D + d) * a.N + n0;
@@ -494,8 +575,36 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
         return total;
     };
 
+    float *mine = ends + warp * (NS + 1) * 32 + lane, *block = ends + LW * (NS + 1) * 32 + lane;
+    // h <- exp(A sum) h + end of a chunk (or of a block's chunks), given how to read it. The decay is applied
+    // as two halves, and not to a state of zero: step by step a growing channel overflows when its
+    // state does, not when its growth over a chunk would.
+    auto fold = [&](auto get) __attribute__((always_inline)) {
+        const f2 half = dup2(0.5f * get(NS));
+#pragma unroll
+        for (int j = 0; j < NS / 2; ++j) {
+            float e0, e1, h0, h1;
+            unpack2(mul2(half, A2[j]), e0, e1);
+            unpack2(h[j], h0, h1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            h[j] = add2(pack2(h0 == 0.0f ? 0.0f : h0 * e0 * e0, h1 == 0.0f ? 0.0f : h1 * e1 * e1), pack2(get(2 * j), get(2 * j + 1)));
+        }
+    };
+    auto fold_warps = [&](int w0, int w1) __attribute__((always_inline)) {
+        float total = 0.0f;
+        for (int w = w0; w < w1; ++w) {
+            const float *e = ends + w * (NS + 1) * 32 + lane;
+            fold([&](int k) { return e[k * 32]; });
+            total += e[NS * 32];
+        }
+        return total;
+    };
+    auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NS / 2; ++j) h[j] = 0;
+    };
     if (chunks > 1) {
-        float *mine = ends + warp * (NS + 1) * 32 + lane, *block = ends + LW * (NS + 1) * 32 + lane;
         auto put = [&](float *to, float total) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NS / 2; ++j) {
@@ -506,58 +615,37 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
             }
             to[NS * 32] = total;
         };
-        // h <- exp(A sum) h + end of a chunk (or of a block's chunks), given how to read it. The decay is applied
-        // as two halves, and not to a state of zero: step by step a growing channel overflows when its
-        // state does, not when its growth over a chunk would.
-        auto fold = [&](auto get) __attribute__((always_inline)) {
-            const f2 half = dup2(0.5f * get(NS));
-#pragma unroll
-            for (int j = 0; j < NS / 2; ++j) {
-                float e0, e1, h0, h1;
-                unpack2(mul2(half, A2[j]), e0, e1);
-                unpack2(h[j], h0, h1);
-                e0 = ex2(e0);
-                e1 = ex2(e1);
-                h[j] = add2(pack2(h0 == 0.0f ? 0.0f : h0 * e0 * e0, h1 == 0.0f ? 0.0f : h1 * e1 * e1), pack2(get(2 * j), get(2 * j + 1)));
-            }
-        };
-        float total = 0.0f;
-        if (chunk < chunks - 1) total = pass(std::false_type{});
-        put(mine, total);
+        put(mine, chunk < chunks - 1 ? pass(std::false_type{}) : 0.0f);
         __syncthreads();
-        auto fold_warps = [&](int w0, int w1) __attribute__((always_inline)) {
-            for (int w = w0; w < w1; ++w) {
-                const float *e = ends + w * (NS + 1) * 32 + lane;
-                fold([&](int k) { return e[k * 32]; });
-                total += e[NS * 32];
-            }
-        };
         if (a.ranks > 1) {  // one channel tile per block
             if (warp == LW - 1 && rank < a.ranks - 1) {
-                total = 0.0f;
-#pragma unroll
-                for (int j = 0; j < NS / 2; ++j) h[j] = 0;
-                fold_warps(0, LW);
-                put(block, total);
+                clear();
+                put(block, fold_warps(0, LW));
             }
             nb::cluster_sync();
-#pragma unroll
-            for (int j = 0; j < NS / 2; ++j) h[j] = 0;
-            const uint32_t e = (uint32_t)__cvta_generic_to_shared(block);
-            for (int q = 0; q < rank; ++q) fold([&](int k) { return nb::ld_cluster(e + k * 128, q); });
-        } else {
-#pragma unroll
-            for (int j = 0; j < NS / 2; ++j) h[j] = 0;
         }
+        // the state before the chunk
+        clear();
+        const uint32_t e = (uint32_t)__cvta_generic_to_shared(block);
+        for (int q = 0; q < rank; ++q) fold([&](int k) { return nb::ld_cluster(e + k * 128, q); });
         fold_warps(warp - warp % a.tw, warp);
         if (chunk == 0 && a.state_in) load_states(a.state_in + at, h);
         pass(std::true_type{});
+    } else {
+        pass(std::true_type{});
+    }
+
+    {
+        float lo, hi;
+        unpack2(h[NS / 2 - 1], lo, hi);
+        const uint32_t hit = __ballot_sync(0xffffffffu, on && n0 + NS > a.N && !(hi == 0.0f));
+        if (hit) run_again<T, LPC, NS, U>(a, hit, h);
+    }
+    if (chunks > 1) {
         // no block leaves while another reads its shared memory; and no chunk writes a state that is to replace
         // the one before it while the first chunk may still read that
         if (a.ranks > 1) nb::cluster_sync();
         else __syncthreads();
-    } else {
-        pass(std::true_type{});
     }
     if (a.state_out && on && chunk == chunks - 1) {
 #pragma unroll

@@ -278,8 +278,9 @@ struct Place {
 };
 
 // States past N fill up a lane with zeros. Times an infinite input or step that is a NaN, which stays, in all of them
-// alike, and goes into the outputs. The channels of the lanes in `hit` were left with one: they run once more, row
-// by row from the stream's first one and with their own states alone, writing the chunk's outputs. (64 streams x 200
+// alike, and goes into the outputs. Channels that were left with one (or whose infinite state cannot be folded over
+// chunks), those of the lanes in `hit`, run once more, row by row from the stream's first one and with their own
+// states alone, writing the chunk's outputs. (64 streams x 200
 // rows, 1024 channels: states past N kept out of every row's sum by a condition cost 4 to 12 %, a test in every tile 1 to
 // 6 %, this nothing. It keeps nothing in registers while the kernel's own passes run, which have none left.)
 template <typename T, int LPC, int NS, int U>
@@ -578,14 +579,20 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
     float *mine = ends + warp * (NS + 1) * 32 + lane, *block = ends + LW * (NS + 1) * 32 + lane;
     // h <- exp(A sum) h + end of a chunk (or of a block's chunks), given how to read it. The decay is applied
     // as two halves, and not to a state of zero: step by step a growing channel overflows when its
-    // state does, not when its growth over a chunk would.
+    // state does, not when its growth over a chunk would. An infinite state stays so row by row, but times a
+    // chunk's decay of zero it is a NaN; and infinite steps leave no sum. Such a channel is `odd`.
+    bool odd = false;
+    __shared__ uint8_t odds[32 * LW_MAX];  // kept there while the rows run
     auto fold = [&](auto get) __attribute__((always_inline)) {
-        const f2 half = dup2(0.5f * get(NS));
+        const float sum = get(NS);
+        const f2 half = dup2(0.5f * sum);
+        odd |= fabsf(sum) == INFINITY;
 #pragma unroll
         for (int j = 0; j < NS / 2; ++j) {
             float e0, e1, h0, h1;
             unpack2(mul2(half, A2[j]), e0, e1);
             unpack2(h[j], h0, h1);
+            odd |= fabsf(h0) == INFINITY || fabsf(h1) == INFINITY;
             e0 = ex2(e0);
             e1 = ex2(e1);
             h[j] = add2(pack2(h0 == 0.0f ? 0.0f : h0 * e0 * e0, h1 == 0.0f ? 0.0f : h1 * e1 * e1), pack2(get(2 * j), get(2 * j + 1)));
@@ -620,15 +627,18 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
         if (a.ranks > 1) {  // one channel tile per block
             if (warp == LW - 1 && rank < a.ranks - 1) {
                 clear();
-                put(block, fold_warps(0, LW));
+                const float total = fold_warps(0, LW);
+                put(block, odd ? INFINITY : total);
             }
             nb::cluster_sync();
         }
         // the state before the chunk
         clear();
+        odd = false;
         const uint32_t e = (uint32_t)__cvta_generic_to_shared(block);
         for (int q = 0; q < rank; ++q) fold([&](int k) { return nb::ld_cluster(e + k * 128, q); });
         fold_warps(warp - warp % a.tw, warp);
+        odds[threadIdx.x] = odd;
         if (chunk == 0 && a.state_in) load_states(a.state_in + at, h);
         pass(std::true_type{});
     } else {
@@ -638,7 +648,7 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
     {
         float lo, hi;
         unpack2(h[NS / 2 - 1], lo, hi);
-        const uint32_t hit = __ballot_sync(0xffffffffu, on && n0 + NS > a.N && !(hi == 0.0f));
+        const uint32_t hit = __ballot_sync(0xffffffffu, on && ((chunks > 1 && odds[threadIdx.x]) || (n0 + NS > a.N && !(hi == 0.0f))));
         if (hit) run_again<T, LPC, NS, U>(a, hit, h);
     }
     if (chunks > 1) {

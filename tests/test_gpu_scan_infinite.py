@@ -72,3 +72,29 @@ def test_infinite_inputs_of_padded_states_where_time_is_cut(c, N, D):
     for s, odd in ((0, (3, 4)), (1, (5,)), (2, (6,)), (3, ())):
         keep = [d for d in range(D) if d not in odd]
         assert torch.equal(y[s][:, keep], clean[s][:, keep]) and torch.equal(h[s][keep], hc[s][keep])
+
+
+@pytest.mark.filterwarnings("ignore:.*invalid value")
+@pytest.mark.parametrize("c,N,D", [(70, 16, 40), (300, 16, 40), (300, 12, 40), (300, 24, 40), (200, 100, 24), (1100, 16, 32), (2500, 8, 40), (700, 64, 24)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_infinite_states_where_time_is_cut(c, N, D, in_place):
+    """Infinite states stay so through any number of decays that are not 0, wherever the rows are cut into
+    chunks; so do those that an infinite input, or an infinite step, makes on the way. Other channels keep their bits."""
+    rng = np.random.default_rng(c + N)
+    S = 2
+    g = positive(rng, S, c, D, N, "f32")
+    clean, hc = scan(g, "f32")
+    g["state"] = g["state"].clone()
+    g["state"][0, 3, 0], g["state"][1, 4, N - 1] = float("inf"), -float("inf")
+    x, dt = g["x"].clone(), g["dt"].clone()
+    x[0, c // 3, 11], x[1, 2, 12] = float("inf"), -float("inf")
+    dt[0, c // 2, 13], x[0, c // 2, 13] = float("inf"), 1.0
+    g = dict(g, x=x, dt=dt)
+    wy, wh, ey, eh = want_of(g)
+    y, h = scan(g, "f32", state_out="same" if in_place else "new")
+    assert np.isinf(wy[0, :, 3]).all() and np.isinf(wy[1, :, 4]).all() and np.isinf(wh[0, 13]).all()
+    compare(R.f64(y), wy, ey, "f32", "y")
+    compare(R.f64(h), wh, eh, "f32", "state")
+    for s, odd in ((0, (3, 11, 13)), (1, (4, 12))):
+        keep = [d for d in range(D) if d not in odd]
+        assert torch.equal(y[s][:, keep], clean[s][:, keep]) and torch.equal(h[s][keep], hc[s][keep])

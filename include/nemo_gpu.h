@@ -199,7 +199,8 @@ int nemo_gemm_mxfp4(const nemo_gemm_mxfp4_args_t *a, void *stream);
    Stream s has lens[s] rows (device ints, taken into 0..c; NULL: c each); rows of y behind its last
    one are left as they were. hist_in [streams][taps-1][D] (NULL: zeros) holds the rows before this
    call's, hist_out the last taps - 1 rows of u after it (NULL: not kept); they may be the same
-   buffer. taps 1..8, c up to 2^30; act NEMO_ACT_NONE or NEMO_ACT_SILU. One row per stream is the single-token form. */
+   buffer. Rows of y must not overlap (refused where it shows: c rows a stream, or with lens one).
+   taps 1..8, c up to 2^30; act NEMO_ACT_NONE or NEMO_ACT_SILU. One row per stream is the single-token form. */
 typedef struct {
     const void *x;
     int64_t x_ld, x_sstride;
@@ -223,7 +224,8 @@ int nemo_causal_conv(const nemo_causal_conv_args_t *a, void *stream);
    z, skip and dt_bias may be NULL (no gate, 0, 0). Rows of B and C hold groups * N elements. Stream s
    has lens[s] rows (device ints, taken into 0..c; NULL: c each); rows of y behind its last one are
    left as they were. state_in [streams][D][N] (NULL: zeros), state_out the state after the last row
-   (of no rows: the state before; NULL: not kept); they may be the same buffer. N 1..128, D up to
+   (of no rows: the state before; NULL: not kept); they may be the same buffer. Rows of y must not
+   overlap (refused where it shows: c rows a stream, or with lens one). N 1..128, D up to
    2^24 and a multiple of groups, c up to 2^30. x, dt, z, B and C rows behind a stream's last one are
    not used, but may be read. One row per stream is the single-token form. */
 typedef struct {

@@ -105,6 +105,7 @@ __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepc
 extern "C" int nb_set_error(const char *fmt, ...);
 extern "C" int nb_pdl_enabled(void);
 extern "C" int nb_smem_attr(const void *func, size_t bytes);
+extern "C" int nb_rows_overlap(int64_t streams, int64_t sstride, int64_t rows, int64_t ld, int64_t width);
 
 namespace nb {
 // Launch with programmatic dependent launch: the grid may be scheduled while its predecessor in

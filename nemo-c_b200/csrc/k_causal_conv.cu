@@ -213,6 +213,9 @@ extern "C" int nemo_causal_conv(const nemo_causal_conv_args_t *p, void *stream) 
     if (p->streams == 0 || p->D == 0) return 0;
     if (!p->w || (p->c > 0 && (!p->x || !p->y))) return nb_set_error("nemo_causal_conv: null pointer");
     if (p->c > 1 && (p->x_ld < p->D || p->y_ld < p->D)) return nb_set_error("nemo_causal_conv: row pitches below D=%d", p->D);
+    // (with lens the rows written are known on the device alone: one row a stream is looked at, then)
+    if (nb_rows_overlap(p->streams, p->y_sstride, p->lens && p->c > 1 ? 1 : p->c, p->y_ld, p->D))
+        return nb_set_error("nemo_causal_conv: rows of y overlap (y_sstride=%lld)", (long long)p->y_sstride);
     const int es = nb::elt_size(p->elt);
     const uintptr_t ptrs = (uintptr_t)p->x | (uintptr_t)p->y | (uintptr_t)p->hist_in | (uintptr_t)p->hist_out;
     if (ptrs % es || ((uintptr_t)p->w | (uintptr_t)p->bias) % 4) return nb_set_error("nemo_causal_conv: buffers must be aligned to their type");

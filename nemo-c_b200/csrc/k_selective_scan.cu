@@ -773,6 +773,9 @@ extern "C" int nemo_selective_scan(const nemo_selective_scan_args_t *p, void *st
     if (!p->A || (p->c > 0 && (!p->x || !p->dt || !p->B || !p->C || !p->y))) return nb_set_error("nemo_selective_scan: null pointer");
     if (p->c > 1 && (p->x_ld < p->D || p->dt_ld < p->D || p->y_ld < p->D || (p->z && p->z_ld < p->D) || p->bc_ld < (int64_t)p->groups * p->N))
         return nb_set_error("nemo_selective_scan: row pitches below the row's elements");
+    // (with lens the rows written are known on the device alone: one row a stream is looked at, then)
+    if (nb_rows_overlap(p->streams, p->y_sstride, p->lens && p->c > 1 ? 1 : p->c, p->y_ld, p->D))
+        return nb_set_error("nemo_selective_scan: rows of y overlap (y_sstride=%lld)", (long long)p->y_sstride);
     const int es = nb::elt_size(p->elt);
     if (((uintptr_t)p->x | (uintptr_t)p->dt | (uintptr_t)p->z | (uintptr_t)p->B | (uintptr_t)p->C | (uintptr_t)p->y) % es ||
         ((uintptr_t)p->A | (uintptr_t)p->skip | (uintptr_t)p->dt_bias | (uintptr_t)p->state_in | (uintptr_t)p->state_out) % 4)

@@ -55,6 +55,22 @@ extern "C" uint64_t nb_graph_kernel_nodes(cudaGraph_t g) {
     return k;
 }
 
+// Whether two of the rows [s * sstride + t * ld, + width), s < streams, t < rows, share an element; rows of one stream
+// do not (ld >= width where there are two). One nested in the other, streams in rows or rows in streams, is
+// seen at once; other strides are looked at one difference of streams at a time.
+extern "C" int nb_rows_overlap(int64_t streams, int64_t sstride, int64_t rows, int64_t ld, int64_t width) {
+    typedef __int128 wide;
+    if (streams < 2 || rows < 1 || width < 1) return 0;
+    const wide step = sstride < 0 ? -(wide)sstride : sstride, extent = (wide)(rows - 1) * ld + width;
+    if (step < width) return 1;
+    if (step >= extent || (wide)ld >= (streams - 1) * step + width) return 0;
+    for (int64_t i = 1; i < streams && i * step < extent; ++i) {
+        const wide t = i * step / ld, rest = i * step % ld;  // this far apart, rows t and t + 1 come nearest
+        if ((t < rows && rest < width) || (t + 1 < rows && ld - rest < width)) return 1;
+    }
+    return 0;
+}
+
 // Raise a kernel's dynamic shared-memory limit to at least `bytes` on the current device. The
 // attribute belongs to the device, so the largest value set so far is kept per (kernel, device),
 // under a lock: a second device, or a thread on another device, sets its own.

@@ -45,6 +45,7 @@ namespace {
 constexpr int BM = 128;   // weight rows per tile
 constexpr int BKB = 128;  // code bytes per row and stage: 256 columns of k, one swizzle span
 constexpr int ATOM = 512; // bytes of one scale tile (128 rows x 128 columns of k)
+constexpr int ERR = 11;   // codes of waits that gave up: a free stage, a free accumulator, a stage's data, a unit's products
 
 struct MxArgs {
     const uint8_t *as, *ws;  // scales
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
                 __syncwarp();
             }
             if (!ok) {
-                if (!flags[0]) { flags[0] = 1; atomicExch(p.err, 5); }
+                if (!flags[0]) { flags[0] = 1; atomicExch(p.err, ERR + 0); }
                 break;
             }
         }
@@ -327,13 +328,13 @@ __global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
                 const int q = t * WT + i;
                 if (q >= C::SLOTS && !sm100::mbar_wait(&acc_empty[q % C::SLOTS], ((q / C::SLOTS) - 1) & 1)) ok = false;
             }
-            if (!__all_sync(0xffffffffu, ok)) { flags[0] = 1; atomicExch(p.err, 6); break; }
+            if (!__all_sync(0xffffffffu, ok)) { flags[0] = 1; atomicExch(p.err, ERR + 1); break; }
             sm100::tc_fence_after();
             // activation tiles of 64 rows: the second one of a scale tile (128 rows) finds its scales two columns on
             const int sb_at = WT * 8 + (BN == 64 ? u % p.n_mtiles % 2 * 2 : 0);
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % C::STAGES;
-                if (!__all_sync(0xffffffffu, sm100::mbar_wait(&full[s], (it / C::STAGES) & 1))) { flags[0] = 1; atomicExch(p.err, 7); break; }
+                if (!__all_sync(0xffffffffu, sm100::mbar_wait(&full[s], (it / C::STAGES) & 1))) { flags[0] = 1; atomicExch(p.err, ERR + 2); break; }
                 sm100::tc_fence_after();
                 const uint32_t st = sm100::smem_u32(stages + s * C::STAGE);
                 const uint32_t sc = tmem + C::SLOTS * BN + s * C::SC_COLS;
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < WT; ++i)
                 if (!sm100::mbar_wait(&acc_full[(t * WT + i) % C::SLOTS], ((t * WT + i) / C::SLOTS) & 1)) good = false;
-            if (!good) { flags[1 + group] = 1; flags[0] = 1; atomicExch(p.err, 8); }
+            if (!good) { flags[1 + group] = 1; flags[0] = 1; atomicExch(p.err, ERR + 3); }
             // the group's flag is written only by its threads before this barrier: all of them decide alike
             sm100::named_barrier(1 + group, 256);
             if (flags[1 + group]) break;

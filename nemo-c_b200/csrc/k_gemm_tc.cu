@@ -1210,6 +1210,9 @@ extern "C" int *nb_tc_error_ptr(void) {
     return p;
 }
 
+// What recorded a code in the error word: 1..8 this file's GEMMs, 9 and 10 the self-test, 11..14 the 4-bit product.
+extern "C" const char *nb_tc_error_name(int code) { return code >= 11 ? "4-bit product" : code >= 9 ? "wait self-test" : "tensor-core GEMM"; }
+
 extern "C" int nemo_gpu_check_device_errors(void) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_tc_error, sizeof v) != cudaSuccess) return nb_set_error("cannot read the device error flag");
@@ -1217,7 +1220,7 @@ extern "C" int nemo_gpu_check_device_errors(void) {
         const int z = 0;
         cudaMemcpyToSymbol(g_tc_error, &z, sizeof z);  // reported once
         g_tc_error_reports.fetch_add(1);
-        return nb_set_error("%s: a bounded device wait gave up (code %d)", v >= 9 ? "wait self-test" : "tensor-core GEMM", v);
+        return nb_set_error("%s: a bounded device wait gave up (code %d)", nb_tc_error_name(v), v);
     }
     const int a = nb_attention_device_error();
     if (a < 0) return nb_set_error("cannot read the attention error flag");

@@ -62,6 +62,8 @@ struct Cfg {
     // Epilogue groups of 8 warps, which take units in turn: two where units are large and many, so that one
     // group's activations run beside the other's loads and stores (the registers of GLU allow one)
     static constexpr int GROUPS = BN == 128 && WT == 1 ? 2 : 1, THREADS = 64 + 256 * GROUPS;
+    // k split over a cluster: not with tiles of 128 rows, which are only taken where tiles of 64 would outnumber the SMs
+    static constexpr bool SPLIT = BN < 128;
     static constexpr int W_BYTES = BM * BKB, A_BYTES = BN * BKB;
     static constexpr int WS_OFF = WT * W_BYTES + A_BYTES;      // scales: 2 atoms per weight tile, 2 for the activations
     static constexpr int STAGE = WS_OFF + (WT + 1) * 2 * ATOM;
@@ -76,7 +78,7 @@ struct Cfg {
     static_assert(SMEM <= 232448, "shared memory");
     static_assert(COLS <= 512, "tensor memory");
     static_assert(STAGE % 1024 == 0, "swizzled tiles start on 1 KB");
-    static_assert(WT * BN * BM * 4 <= STAGES * STAGE, "partial tiles reuse the stages");
+    static_assert(!SPLIT || WT * BN * BM * 4 <= STAGES * STAGE, "partial tiles reuse the stages");
 };
 
 __device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
@@ -274,8 +276,9 @@ __global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
     nb::pdl_wait();
 
     constexpr bool glu = WT == 2;
-    const int rank = p.splits > 1 ? (int)nb::cluster_rank() : 0;
-    const int u0 = p.splits > 1 ? blockIdx.x / p.splits : blockIdx.x, ustep = p.splits > 1 ? p.units : gridDim.x;
+    const bool split = C::SPLIT && p.splits > 1;
+    const int rank = split ? (int)nb::cluster_rank() : 0;
+    const int u0 = split ? blockIdx.x / p.splits : blockIdx.x, ustep = split ? p.units : gridDim.x;
     const int kb0 = rank * p.kb_per_split, kb1 = min(p.kblocks, kb0 + p.kb_per_split);
     // first weight row of tile i of unit u
     auto wrow = [&](int wt, int i) { return wt * BM + (i ? p.N / 2 : 0); };
@@ -400,7 +403,7 @@ __global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
             if (flags[1 + group]) break;
             sm100::tc_fence_after();
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
-            if (p.splits > 1) {  // partial tiles to shared memory: [tile][column][lane]
+            if (split) {  // partial tiles to shared memory: [tile][column][lane]
                 float *part = (float *)stages;
 #pragma unroll
                 for (int i = 0; i < WT; ++i)
@@ -479,7 +482,7 @@ __global__ void __launch_bounds__(Cfg<BN, WT>::THREADS, 1)
         }
     }
     __syncwarp();
-    if (p.splits > 1) {
+    if (split) {
         // one unit per cluster: each rank adds and finishes its share of the columns
         __syncthreads();
         nb::cluster_sync();
@@ -573,12 +576,12 @@ int run(const nemo_gemm_mxfp4_args_t *a, cudaStream_t st) {
     if (units > 0x3fffffff) return nb_set_error("nemo_gemm_mxfp4: too many tiles");
     p.units = (int)units;
     // k is split over a cluster while the CTAs fit the SMs and the k-blocks saved (0.16 us each) pay for
-    // joining the partial tiles (about 1 us + 7 ns per column and rank): M = 1, N = 1024, K = 4096 takes 5.9 us
-    // whole and 4.9 us in 8 parts, but M = 7, N = 2048, K = 1024 4.0 and 5.3 us, and M = 256, N = 1024, K = 4096 7.5
-    // and 14.2 us.
+    // joining the partial tiles (about 1 us + 7 ns per column and rank). M = 1, N = 1024, K = 4096: 5.9 us whole, 5.0 us
+    // in the 4 parts that this takes, 4.6 us in 8; M = 1, N = 256, K = 8192: 8.9 us whole, 4.7 us in 8. Against: M = 7,
+    // N = 2048, K = 1024 3.5 us whole, 4.5 us in 2 or 4; M = 256, N = 1024, K = 4096 6.5 us whole, 7.7 and 6.9 us.
     int splits = 1;
     float best = 0.16f * p.kblocks;
-    for (int s = 2; s <= 8 && p.units * s <= sms && s <= p.kblocks; s *= 2) {
+    for (int s = 2; C::SPLIT && s <= 8 && p.units * s <= sms && s <= p.kblocks; s *= 2) {
         const int per = (p.kblocks + s - 1) / s;
         const float cost = 0.16f * per + 1.0f + 0.007f * BN * s;
         if (cost < best && (s - 1) * per < p.kblocks) {  // every rank has k-blocks

@@ -31,10 +31,12 @@ struct ScanArgs {
     int lw, tw, ranks; // runs: warps in a block, chunks of time in it, blocks of a cluster
 };
 
-// Over [-1, 0] the special-function units' 2^x is within 1.4e-7 of the exact value, and too small by 5e-9 (at
-// -1e-4) to 2.6e-8 (at -0.03) of it on average (measured): less than a step of fp32, but the same way for
-// every row of a long memory. 2^-26 in the exponent, 1.03e-8 of the value, leaves half of that at most where
-// memories are long; it is too little to turn a decay of 1 into anything else.
+// The special-function units' 2^x makes decays e^-v too small on average: by 5.1e-9 to 8.4e-9 of the value for v from
+// 1e-5 to 3e-3, 2.4e-8 to 2.5e-8 from 3e-3 to 0.03, 1.6e-8 to 0.3, 2.5e-8 to 3 (a million values each; single values
+// are within 1.5e-7 up to 1). That is less than a step of fp32, but the same way in every row of a long memory.
+// With 2^-26 in the exponent, 1.03e-8 of the value, they are too large by 1.9e-9 to 5.3e-9 up to 3e-3, and too
+// small by 1.5e-8 to 0.03, 6e-9 to 0.3 and 1.5e-8 to 3. It is too little to turn a decay of 1 into anything else.
+// (Chunks are folded without it: two decays each, against one a row.)
 constexpr float EVEN = 0x1p-26f;
 
 // log(1 + e^v) = max(v, 0) + log1p(e), e = exp(-|v|) <= 1, and log1p(e) = 2 artanh(e / (2 + e)): the
@@ -218,9 +220,9 @@ __device__ __forceinline__ f2 softplus2(f2 v) {
 // and C, shared by the warp's channels, pass through shared memory. A warp runs one chunk of rows of its
 // channels. Where the channels alone do not fill the GPU, time is cut as well: TW warps of a block
 // and R blocks of a cluster hold chunks of the same channels. Each chunk but the last finds the state
-// it ends in when started from zero, and the sum of its steps (all chunks start at once; the first
-// one starts from the true state and is done). A chunk's true first state is then folded from those
-// before it, h <- exp(A sum of steps) h + end, and the chunks run again from it, writing y. Nothing
+// it ends in when started from zero (the first one from the true state), and the sum of its steps, all
+// at once. A chunk's true first state is then folded from those before it, h <- exp(A sum of steps) h + end,
+// and all chunks run again, from their true first states, writing y. Nothing
 // but shared memory is needed for that, and the order of the sums is fixed.
 //
 // Measured: 64 streams x 200 rows x 2048 channels, 16 states, bf16: 165 us, of which the special-function units

@@ -581,37 +581,51 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
     float *mine = ends + warp * (NS + 1) * 32 + lane, *block = ends + LW * (NS + 1) * 32 + lane;
     // h <- exp(A sum) h + end of a chunk (or of a block's chunks), given how to read it. The decay is applied
     // as two halves, and not to a state of zero: step by step a growing channel overflows when its
-    // state does, not when its growth over a chunk would. An infinite state stays so row by row, but times a
-    // chunk's decay of zero it is a NaN; and infinite steps leave no sum. Such a channel is `odd`.
+    // state does, not when its growth over a chunk would.
+    // An infinite state stays so row by row, but times a chunk's decay of zero it is a NaN; and infinite steps leave no
+    // sum. Such a channel is `odd`; whether it is, is looked at (CHECK) only where a state that is not finite came out.
     bool odd = false;
     __shared__ uint8_t odds[32 * LW_MAX];  // kept there while the rows run
-    auto fold = [&](auto get) __attribute__((always_inline)) {
+    auto fold = [&](auto get, auto check) __attribute__((always_inline)) {
+        constexpr bool CHECK = decltype(check)::value;
         const float sum = get(NS);
         const f2 half = dup2(0.5f * sum);
-        odd |= fabsf(sum) == INFINITY;
+        if (CHECK) odd |= fabsf(sum) == INFINITY;
 #pragma unroll
         for (int j = 0; j < NS / 2; ++j) {
             float e0, e1, h0, h1;
             unpack2(mul2(half, A2[j]), e0, e1);
             unpack2(h[j], h0, h1);
-            odd |= fabsf(h0) == INFINITY || fabsf(h1) == INFINITY;
+            if (CHECK) odd |= fabsf(h0) == INFINITY || fabsf(h1) == INFINITY;
             e0 = ex2(e0);
             e1 = ex2(e1);
             h[j] = add2(pack2(h0 == 0.0f ? 0.0f : h0 * e0 * e0, h1 == 0.0f ? 0.0f : h1 * e1 * e1), pack2(get(2 * j), get(2 * j + 1)));
         }
     };
-    auto fold_warps = [&](int w0, int w1) __attribute__((always_inline)) {
+    // from a state of zero over the blocks before `r` and the chunks w0 .. w1 - 1 of this one; the sum of the latter
+    auto fold_all = [&](int r, int w0, int w1, auto check) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NS / 2; ++j) h[j] = 0;
+        const uint32_t b = (uint32_t)__cvta_generic_to_shared(block);
+        for (int q = 0; q < r; ++q) fold([&](int k) { return nb::ld_cluster(b + k * 128, q); }, check);
         float total = 0.0f;
         for (int w = w0; w < w1; ++w) {
             const float *e = ends + w * (NS + 1) * 32 + lane;
-            fold([&](int k) { return e[k * 32]; });
+            fold([&](int k) { return e[k * 32]; }, check);
             total += e[NS * 32];
         }
         return total;
     };
-    auto clear = [&]() __attribute__((always_inline)) {
+    auto fold_odd = [&](int r, int w0, int w1) __attribute__((always_inline)) {
+        const float total = fold_all(r, w0, w1, std::false_type{});
+        f2 wild = 0;
 #pragma unroll
-        for (int j = 0; j < NS / 2; ++j) h[j] = 0;
+        for (int j = 0; j < NS / 2; ++j) wild = fma2(h[j], dup2(0.0f), wild);
+        float lo, hi;
+        unpack2(wild, lo, hi);
+        odd = false;
+        if (lo + hi != 0.0f) fold_all(r, w0, w1, std::true_type{});  // the same states again
+        return total;
     };
     if (chunks > 1) {
         auto put = [&](float *to, float total) __attribute__((always_inline)) {
@@ -628,18 +642,12 @@ __global__ void __launch_bounds__(32 * LW_MAX, 2) scan_long_kernel(const __grid_
         __syncthreads();
         if (a.ranks > 1) {  // one channel tile per block
             if (warp == LW - 1 && rank < a.ranks - 1) {
-                clear();
-                const float total = fold_warps(0, LW);
+                const float total = fold_odd(0, 0, LW);
                 put(block, odd ? INFINITY : total);
             }
             nb::cluster_sync();
         }
-        // the state before the chunk
-        clear();
-        odd = false;
-        const uint32_t e = (uint32_t)__cvta_generic_to_shared(block);
-        for (int q = 0; q < rank; ++q) fold([&](int k) { return nb::ld_cluster(e + k * 128, q); });
-        fold_warps(warp - warp % a.tw, warp);
+        fold_odd(rank, warp - warp % a.tw, warp);  // the state before the chunk
         odds[threadIdx.x] = odd;
         if (chunk == 0 && a.state_in) load_states(a.state_in + at, h);
         pass(std::true_type{});

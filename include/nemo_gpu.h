@@ -148,13 +148,13 @@ int nemo_joint_argmax(const float *enc, int64_t enc_ld, const float *pred, int64
                       const float *bias, int V, int H, int rows, int *out_idx, float *out_val, void *stream);
 
 /* ---- operators of streaming state-space layers -------------------------------------------------
-   The reference has none of these: they serve checkpoints whose projections are held in 4 bits and
-   whose sequence mixer carries a fixed state (causal convolution + selective scan) instead of a K/V
-   window. Activations may be fp32, bf16 or fp16 (NEMO_ELT_*); sums and states are fp32 and a value
-   is rounded once, to nearest even, where it is stored. Values, small tensors and states need the
-   alignment of their type; rows whose base and pitch are 16-byte aligned are moved 16 bytes at a
-   time. Buffers that are written must not overlap others unless stated. Nothing is allocated and
-   nothing synchronises; calls may be captured into graphs and may run on several streams at once. */
+   The reference has none of these: they serve layers, built by the caller, whose projections are held
+   in 4 bits and whose sequence mixer carries a fixed state (causal convolution + selective scan)
+   instead of a K/V window; nemoasr_open reads no such checkpoints. Activations may be fp32, bf16 or
+   fp16 (NEMO_ELT_*); sums and states are fp32 and a value is rounded once, to nearest even, where it
+   is stored. Values, small tensors and states need the alignment of their type; rows whose base and
+   pitch are 16-byte aligned are moved 16 bytes at a time. Buffers that are written must not overlap
+   others unless stated. Nothing is allocated and nothing synchronises; calls may be captured into graphs and may run on several streams at once. */
 enum { NEMO_ELT_F32 = 0, NEMO_ELT_BF16 = 1, NEMO_ELT_F16 = 2 };
 
 /* MXFP4 rows. A block is 32 consecutive columns of a row; its scale is 2^e with e = floor(log2 of

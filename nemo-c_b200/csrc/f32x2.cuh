@@ -39,7 +39,7 @@ __device__ __forceinline__ float rcp(float v) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 
-// 1 / (1 + e^-v): an infinite exponential gives 0, a NaN stays one
+// 1 / (1 + e^-v): below v = -87.3, where it is less than 2^-126, it is 0; a NaN stays one
 __device__ __forceinline__ float sigmoid_fast(float v) { return rcp(1.0f + ex2(v * -LOG2E)); }
 __device__ __forceinline__ f2 sigmoid2(f2 v) {
     float a, b;

@@ -21,9 +21,9 @@
 // the epilogue. Every wait on a barrier is bounded: on a timeout the CTA records an
 // error, takes part in the remaining cluster barriers and unwinds.
 //
-// Measured (tensor products alone): 14322 x 1024 x 4096 to fp32 39.6 to 41.7 us (2.9 PFLOP/s, 1.8 times the measured
-// bf16 rate), 8192 cubed 245 us (4.5 PFLOP/s), 1792 x 4096 x 1024 with SiLU to bf16 12.4 us, one row by
-// 1024 x 4096 5.2 us. What held it back, in the order found: the issuing thread (descriptors computed for each
+// Measured (tensor products alone): 14322 x 1024 x 4096 to fp32 38.8 to 41.7 us (2.9 PFLOP/s or more, 1.8 times the
+// measured bf16 rate), accumulating 67 us; 8192 cubed 248 us (4.4 PFLOP/s); 1792 x 4096 x 1024 to bf16 with SiLU 12.2 us,
+// with GLU 10.1 us; one row by 1024 x 4096 5.0 us. What held it back, in the order found: the issuing thread (descriptors computed for each
 // MMA in divergent code: 82 us for the first shape; constant words and an unrolled stage 59 us; uniform control
 // flow, so that operands come from uniform registers, 50 us; the same for the loading warp 40 us); then, where k is
 // short, the epilogue: accumulators released as soon as they are in registers, two groups of epilogue

@@ -70,9 +70,9 @@ __device__ __forceinline__ float cooked(uint32_t v) {
 // One row per stream: bound by HBM (8 N bytes of state per channel). A warp owns 32 / LPC channels of
 // SB streams: the streams' rows are taken together, so that SB states are in flight per lane and A is
 // read once for them. What is left above HBM's time is the time between a warp's loads and its stores,
-// so instructions count: 1024 streams of 2048 channels, 16 states, bf16: 63 us (4.5 TB/s, 0.69 of the measured
+// so instructions count: 1024 streams of 2048 channels, 16 states, bf16: 59 us (4.8 TB/s, 0.74 of the measured
 // copy rate) where the same plan with 566 instructions a warp, predicated loads and a shuffle per stream's
-// liveness took 78 us; N = 64, 1024 channels: 120 us, was 184 us.
+// liveness took 78 us; N = 64, 1024 channels: 121 us, was 184 us.
 constexpr int STEP_NT = 128, STEP_SB = 4;
 
 template <typename T, int LPC, bool V4>
@@ -225,9 +225,9 @@ __device__ __forceinline__ f2 softplus2(f2 v) {
 // and all chunks run again, from their true first states, writing y. Nothing
 // but shared memory is needed for that, and the order of the sums is fixed.
 //
-// Measured: 64 streams x 200 rows x 2048 channels, 16 states, bf16: 165 us, of which the special-function units
-// are busy 70 % (their 17 exponentials and more per row and channel: 115 us) and instructions issue 59 %, 140 a row
-// for 32 channels; 16384 rows of one stream, two passes: 467 us (283 us of special functions). Four lanes a
+// Measured: 64 streams x 200 rows x 2048 channels, 16 states, bf16: 163 us, of which the special-function units
+// are busy 69 % (their 17 exponentials and more per row and channel) and instructions issue 51 %, 118 a row
+// for 32 channels; 16384 rows of one stream, two passes: 468 us (70 % and 46 %). Four lanes a
 // channel with rows prepared by other warps in shared memory: 500 us for the latter in one pass, bound by
 // shared memory's 128 bytes a clock (steps, B, C and sums pass through it for every lane).
 constexpr int LW_MAX = 8;  // warps per block: 4 or 8
@@ -284,7 +284,8 @@ struct Place {
 // chunks), those of the lanes in `hit`, run once more, row by row from the stream's first one and with their own
 // states alone, writing the chunk's outputs. (64 streams x 200
 // rows, 1024 channels: states past N kept out of every row's sum by a condition cost 4 to 12 %, a test in every tile 1 to
-// 6 %, this nothing. It keeps nothing in registers while the kernel's own passes run, which have none left.)
+// 6 %, this nothing where no channel needs it, and 1.0 to 1.5 us a row where one does. It keeps nothing in registers while
+// the kernel's own passes run, which have none left.)
 template <typename T, int LPC, int NS, int U>
 __device__ __forceinline__ void run_again(const ScanArgs &a, uint32_t hit, f2 (&h)[NS / 2]) {
     uint32_t block, thread;
@@ -699,8 +700,8 @@ int launch_long(ScanArgs a, cudaStream_t st) {
     int chunks = 1;
     if (a.items < 148 * 5)
         while (chunks < 64 && a.items * chunks < 148 * 32 && chunks * 2 * 32 <= a.c) chunks *= 2;
-    // blocks of four warps spread better where one block need not hold several chunks (64 streams of 200 rows: 170 us,
-    // 192 us with eight)
+    // blocks of four warps spread better where one block need not hold several chunks (64 streams of 200 rows, in
+    // tiles of four: 170 us, 192 us with eight)
     const int LW = a.lw = chunks == 1 ? 4 : 8;
     a.tw = chunks < LW ? chunks : LW;
     a.ranks = chunks / a.tw;
@@ -734,8 +735,8 @@ int launch_long(ScanArgs a, cudaStream_t st) {
 
 template <typename T, int LPC, int NS, bool V4>
 int run_long(const ScanArgs &a, cudaStream_t st) {
-    // asynchronous copies of 16 bytes (8 where a warp has four 16-bit channels) where all rows allow it (recording of 16384 rows: 495 us
-    // without, 485 us with; prompts 347 and 319 us)
+    // asynchronous copies of 16 bytes (8 where a warp has four 16-bit channels) where all rows allow it (in tiles of four rows, recording of
+    // 16384 rows: 495 us without, 485 us with; prompts 347 and 319 us)
     constexpr int E = 16 / sizeof(T);
     const uintptr_t ptrs = (uintptr_t)a.x | (uintptr_t)a.dt | (uintptr_t)a.z | (uintptr_t)a.B | (uintptr_t)a.C;
     const int64_t strides = a.x_ld | a.x_ss | a.dt_ld | a.dt_ss | (a.z ? a.z_ld | a.z_ss : 0) | a.bc_ld | a.bc_ss;

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(STEP_NT, 6) scan_step_kernel(const __grid_cons
                 unpack2(fma2(st2, A2[j], dup2(EVEN)), e0, e1);
                 f2 hh = fma2(pack2(ex2(e0), ex2(e1)), pack2(h[r].v[2 * j], h[r].v[2 * j + 1]),
                              mul2(in2, pack2(to_f32(b[r].v[2 * j]), to_f32(b[r].v[2 * j + 1]))));
-                if (!V4) {  // states past N: see below
+                if (!V4) {  // states past N stay zeros (an infinite input times zero is a NaN)
                     unpack2(hh, e0, e1);
                     hh = pack2(n0 + 2 * j < a.N ? e0 : 0.0f, n0 + 2 * j + 1 < a.N ? e1 : 0.0f);
                 }
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(STEP_NT, 6) scan_step_kernel(const __grid_cons
             sum[r] = lo + hi;
         }
     }
-    if (V4 && !st4) {  // states past N are zeros, but those times an infinite input are NaN
+    if (V4 && !st4) {  // a lane of states past N
 #pragma unroll
         for (int r = 0; r < SB; ++r) sum[r] = 0.0f;
     }
@@ -282,10 +282,10 @@ struct Place {
 // States past N fill up a lane with zeros. Times an infinite input or step that is a NaN, which stays, in all of them
 // alike, and goes into the outputs. Channels that were left with one (or whose infinite state cannot be folded over
 // chunks), those of the lanes in `hit`, run once more, row by row from the stream's first one and with their own
-// states alone, writing the chunk's outputs. (64 streams x 200
-// rows, 1024 channels: states past N kept out of every row's sum by a condition cost 4 to 12 %, a test in every tile 1 to
-// 6 %, this nothing where no channel needs it, and 1.0 to 1.5 us a row where one does. It keeps nothing in registers while
-// the kernel's own passes run, which have none left.)
+// states alone, writing the chunk's outputs. 64 streams x 200 rows, 1024 channels: states past N kept out of every
+// row's sum by a condition cost 4 to 12 %, a test in every tile 1 to 6 %, this nothing where no channel needs it, and 1.0
+// to 1.5 us a row where one does. Its addresses are formed anew: kept in registers while the kernel's own passes
+// run, which have none left, they cost up to 11 %.
 template <typename T, int LPC, int NS, int U>
 __device__ __forceinline__ void run_again(const ScanArgs &a, uint32_t hit, f2 (&h)[NS / 2]) {
     uint32_t block, thread;

@@ -285,7 +285,7 @@ struct Place {
 // states alone, writing the chunk's outputs. 64 streams x 200 rows, 1024 channels: states past N kept out of every
 // row's sum by a condition cost 4 to 12 %, a test in every tile 1 to 6 %, this nothing where no channel needs it, and 1.0
 // to 1.5 us a row where one does. Its addresses are formed anew: kept in registers while the kernel's own passes
-// run, which have none left, they cost up to 11 %.
+// run, which have none left, they cost up to 16 %.
 template <typename T, int LPC, int NS, int U>
 __device__ __forceinline__ void run_again(const ScanArgs &a, uint32_t hit, f2 (&h)[NS / 2]) {
     uint32_t block, thread;
